@@ -108,6 +108,83 @@ int krb_qk_norm_rope_bf16(void *qkv, int S, int HQ, int HKV, int D, const void *
 int krb_attention_prefill_bf16(const void *qkv, void *out, int S, int HQ, int HKV, int D,
                                float scale, int impl, uint32_t *status, void *stream);
 
+/* ---------------------------------------------------------------- paged K/V cache
+ * Operators of the steps after the prompt; no reference counterpart (the reference runs one
+ * prefill).  A cache is two arrays K and V [layers, pages, heads, page_size, head_dim] of
+ * 2-byte elements in device memory of the caller, any order of the outer axes: strides in
+ * elements of (layer, page, head, slot), head_dim contiguous; k, v 16-byte aligned, strides
+ * multiples of 8 whose rows do not overlap.  page_size is a power of two from 8 on, head_dim 64
+ * or 128.  A sequence's tokens live in the pages of its row of a page table (int32 [B,
+ * max_pages], row pitch ldp): position p in page table[p / page_size], slot p % page_size.
+ * Entries behind a sequence's last page are never read.  max_pages * page_size <= 2^30.
+ *
+ * A bad value that only the device sees (an index outside its range, impossible lengths) is
+ * never followed: it sets bit 7 or 8 of *status (may be NULL), and what the call then leaves
+ * out is stated per call. */
+typedef struct krb_kv_cache {
+  void *k, *v;
+  int dtype; /* 0: bf16, 1: fp16 */
+  int layers, pages, heads, page_size, head_dim;
+  int64_t k_stride[4], v_stride[4];
+} krb_kv_cache;
+
+/* Per token n of qkv [N, (HQ+2*HKV)*D] (cache dtype, row pitch ldqkv; HKV = heads, D =
+ * head_dim): optional per-head RMSNorm of the q and k heads (q_norm / k_norm bf16 [D], both or
+ * neither), rotate-half RoPE with row positions[n] of the bf16 tables cos / sin [max_pos, D],
+ * then q -> q_out [N, HQ*D] (row pitch ldq; may be the q columns of qkv itself), and the k and
+ * v heads -> slot slots[n] = page * page_size + offset of `layer`.  Rounds once, at the store.
+ * slots[n] = -1 writes no k and v (a padded token); any other slots must differ from each
+ * other.  A slot outside [-1, pages * page_size) sets bit 8 and writes no k and v; a position
+ * outside [0, max_pos) sets bit 8, writes no k and v and zeros to q.  The form of
+ * krb_qk_norm_rope_bf16 for tokens at any position (one or many per sequence). */
+int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv, int64_t ldqkv,
+                           void *q_out, int64_t ldq, const int64_t *positions,
+                           const int64_t *slots, int N, int HQ, const void *cos_tab,
+                           const void *sin_tab, int max_pos, const void *q_norm,
+                           const void *k_norm, float eps, uint32_t *status, void *stream);
+
+/* Attention of new tokens over the cache.  Sequence b's new tokens are rows q_starts[b] ..
+ * q_starts[b+1]-1 of q and out [N, HQ*D] (row pitches ldq, ldo; cache dtype); kv_lens[b] is its
+ * cached length WITH the new tokens, which are its last T_b positions (append them first).
+ * Every new token sees all positions before the new ones; of the new ones, token i sees those up
+ * to itself (mask NULL: one token, or a chunk of a prompt), or token j where bit j % 32 of word j
+ * / 32 of its mask row is set (uint32 [N, mask_words], row pitch ldm; a tree of drafted
+ * tokens; needs max_q <= 32 * mask_words).  A row that sees nothing gives zeros.  The drafted
+ * tokens' keys and values must be finite where other tokens of the sequence are to be (a masked
+ * infinite value times a zero probability is not a number); slots behind kv_lens[b] may hold
+ * anything.  max_q bounds every T_b, HQ / HKV <= 64, scale > 0.  T_b = 0 is allowed.
+ * A sequence with T_b > max_q, kv_lens[b] < T_b or > max_pages * page_size, or rows outside
+ * [0, N) sets bit 7 and its rows are left as they were, like rows that belong to no sequence.
+ * A page outside [0, pages) sets bit 8 and is read as page 0.
+ * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call
+ * alone until it is done; calls in order on one stream may share one. */
+int krb_attention_paged(const krb_kv_cache *cache, int layer, const void *q, int64_t ldq,
+                        void *out, int64_t ldo, int N, int HQ, const int32_t *page_table,
+                        int64_t ldp, int max_pages, const int32_t *kv_lens,
+                        const int32_t *q_starts, int B, int max_q, const uint32_t *mask,
+                        int64_t ldm, int mask_words, float scale, void *workspace,
+                        size_t workspace_bytes, uint32_t *status, void *stream);
+/* Bytes of krb_attention_paged's workspace for these sizes on the current device (0 and a
+ * message on a bad argument). */
+size_t krb_attention_paged_workspace(const krb_kv_cache *cache, int HQ, int max_q);
+
+/* Copies page src[i] to page dst[i], K and V of all layers, for i < n.  src and dst are HOST
+ * arrays, read before the call returns (inside a stream capture: the captured values).  A page
+ * may be copied to several others; no page may be written twice, or both read and written
+ * (but src[i] == dst[i] is allowed and does nothing). */
+int krb_kv_copy_pages(const krb_kv_cache *cache, const int32_t *src, const int32_t *dst, int n,
+                      void *stream);
+
+/* Keeps the accepted tokens of verified drafts: for each sequence b and i < counts[b], the K and V
+ * rows of position bases[b] + accepted[b][i] move to position bases[b] + i, all layers
+ * (accepted int32 [B, A], row pitch lda; device arrays).  accepted[b] must ascend strictly from
+ * >= 0, so a row is never overwritten before it is read.  A sequence whose counts, bases,
+ * accepted or pages are out of range or order sets bit 8 and is left as it was.  The pages that
+ * two sequences move rows in must differ. */
+int krb_kv_commit(const krb_kv_cache *cache, const int32_t *page_table, int64_t ldp, int max_pages,
+                  const int32_t *bases, const int32_t *accepted, int64_t lda, int A,
+                  const int32_t *counts, int B, uint32_t *status, void *stream);
+
 /* Fused down-GEMM + row-tile relay + Add+RMSNorm on ONE device (tp degree 1):
  *   down = act[S,K] . w_down[H,K]^T (bf16 partial), released to the consumer
  *   warps tile by tile through device counters; sum = resid + down (resid and

@@ -5,6 +5,7 @@ If the library is missing the import of the wrappers fails loudly.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import json
 import os
@@ -21,6 +22,14 @@ c_size_t = ctypes.c_size_t
 c_char_p = ctypes.c_char_p
 c_u64 = ctypes.c_uint64
 c_u32p = ctypes.POINTER(ctypes.c_uint32)
+c_i64 = ctypes.c_int64
+
+
+class KVCacheDesc(ctypes.Structure):
+    """krb_kv_cache of include/kernrelay_b200.h."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("layers", c_int),
+                ("pages", c_int), ("heads", c_int), ("page_size", c_int), ("head_dim", c_int),
+                ("k_stride", ctypes.c_int64 * 4), ("v_stride", ctypes.c_int64 * 4)]
 
 
 def lib_path() -> Path:
@@ -65,6 +74,17 @@ SIGNATURES = [
                                       c_void_p, c_void_p, c_float, c_void_p]),
     ("krb_attention_prefill_bf16", c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                            c_float, c_int, c_void_p, c_void_p]),
+    ("krb_qk_norm_rope_paged", c_int, [c_void_p, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p,
+                                       c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
+                                       c_void_p, c_void_p, c_float, c_void_p, c_void_p]),
+    ("krb_attention_paged", c_int, [c_void_p, c_int, c_void_p, c_i64, c_void_p, c_i64, c_int,
+                                    c_int, c_void_p, c_i64, c_int, c_void_p, c_void_p, c_int,
+                                    c_int, c_void_p, c_i64, c_int, c_float, c_void_p, c_size_t,
+                                    c_void_p, c_void_p]),
+    ("krb_attention_paged_workspace", c_size_t, [c_void_p, c_int, c_int]),
+    ("krb_kv_copy_pages", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    ("krb_kv_commit", c_int, [c_void_p, c_void_p, c_i64, c_int, c_void_p, c_void_p, c_i64, c_int,
+                              c_void_p, c_int, c_void_p, c_void_p]),
     ("krb_relay_down_single", c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_int, c_int, c_int, c_int, c_float, c_int, c_void_p,
                                       c_void_p]),
@@ -131,6 +151,20 @@ def check(rc: int, what: str = ""):
 
 def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _empty(shape, dtype, device, stream):
+    """A tensor that this call's kernels on `stream` use: allocated on that stream, so that the
+    allocator does not hand its memory to another stream's work too early."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _stream(stream):
@@ -261,6 +295,199 @@ def attention(qkv, HQ, HKV, D, scale, impl=0, status=None, stream=None):
     check(lib().krb_attention_prefill_bf16(_ptr(qkv), _ptr(out), S, HQ, HKV, D, scale, impl,
                                            _ptr(status), _stream(stream)), "attention")
     return out
+
+
+# ---------------------------------------------------------------- paged K/V cache
+class KVCache:
+    """A paged K/V cache in the caller's tensors: k and v of the same shape [pages, heads,
+    page_size, head_dim], or [layers, pages, ...], bf16 or fp16, head_dim contiguous, the other
+    axes of any strides (pass `x.transpose(-3, -2)` where the slot axis is stored outside the
+    heads').  page_size: a power of two from 8 on; head_dim 64 or 128.  The handle keeps the
+    tensors; make it once per cache."""
+
+    def __init__(self, k, v):
+        import torch
+        if k.shape != v.shape or k.dim() not in (4, 5):
+            raise KrbError("KVCache: k and v must be [pages, heads, page_size, head_dim] or "
+                           "[layers, pages, heads, page_size, head_dim]")
+        if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+            raise KrbError("KVCache: k and v must both be bf16 or both fp16")
+        if k.device != v.device:
+            raise KrbError("KVCache: k and v on different devices")
+        if k.stride(-1) != 1 or v.stride(-1) != 1:
+            raise KrbError("KVCache: head_dim must be contiguous")
+        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        sizes = ((1,) + tuple(k.shape))[-5:]
+        self.layers, self.pages, self.heads, self.page_size, self.head_dim = sizes
+        strides = [((0,) + tuple(t.stride()))[-5:-1] for t in (k, v)]
+        self.desc = KVCacheDesc(k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16), *sizes,
+                                *((c_i64 * 4)(*s) for s in strides))
+        self.ref = ctypes.addressof(self.desc)
+        self._workspaces = {}  # (HQ, max_q) -> bytes
+
+    def attention_workspace(self, HQ, max_q):
+        """Bytes of attention_paged's workspace (krb_attention_paged_workspace)."""
+        n = self._workspaces.get((HQ, max_q))
+        if n is None:
+            with _on(self.device):
+                n = lib().krb_attention_paged_workspace(self.ref, HQ, max_q)
+            if not n:
+                raise KrbError(lib().krb_last_error().decode(errors="replace"))
+            self._workspaces[HQ, max_q] = n
+        return n
+
+
+def _on(device):
+    """The device that the library's calls run on, where it is not the current one."""
+    import torch
+    if device.type != "cuda" or device.index in (None, torch.cuda.current_device()):
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _want(what, name, t, dtype, device, dim, inner=True):
+    if t.dtype != dtype or t.device != device or t.dim() != dim or (
+            inner and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise KrbError(f"{what}: {name} must be a {dim}-d {dtype} tensor on {device} with its last "
+                       f"axis contiguous, got {t.dim()}-d {t.dtype} on {t.device}, strides "
+                       f"{tuple(t.stride())}")
+
+
+def _pitch(t):
+    """Row pitch of a 2-d tensor (rows that are never stepped over may have any stride)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, k_norm=None,
+                       eps=1e-6, layer=0, out=None, status=None, stream=None):
+    """Per-head norms (optional) and RoPE at positions[n] for the q and k heads of
+    qkv [N, (HQ+2*HKV)*D]; returns the rotated q [N, HQ*D] and writes the k and v heads to slot
+    slots[n] = page * page_size + offset of the cache's `layer` (-1: not written).  positions and
+    slots int64 [N]; cos / sin bf16 [max_pos, D]."""
+    import torch
+    what = "qk_norm_rope_paged"
+    N, D, dev = qkv.shape[0], cache.head_dim, cache.device
+    _want(what, "qkv", qkv, cache.dtype, dev, 2)
+    if qkv.shape[1] != (HQ + 2 * cache.heads) * D:
+        raise KrbError(f"{what}: qkv rows must hold (HQ + 2*HKV) * head_dim values")
+    for name, t in (("positions", positions), ("slots", slots)):
+        _want(what, name, t, torch.int64, dev, 1)
+        if t.shape[0] != N:
+            raise KrbError(f"{what}: {name} must have one entry per row of qkv")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _want(what, name, t, torch.bfloat16, dev, 2)
+        if t.shape != cos.shape or t.shape[1] != D or not t.is_contiguous():
+            raise KrbError(f"{what}: cos and sin must be contiguous [max_pos, head_dim]")
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            _want(what, name, t, torch.bfloat16, dev, 1)
+            if t.shape[0] != D:
+                raise KrbError(f"{what}: {name} must have head_dim values")
+    if status is not None:
+        _want(what, "status", status, torch.int32, dev, 1)
+    with _on(dev):
+        if out is None:
+            out = _empty((N, HQ * D), cache.dtype, dev, stream)
+        else:
+            _want(what, "out", out, cache.dtype, dev, 2)
+            if out.shape != (N, HQ * D):
+                raise KrbError(f"{what}: out must be [N, HQ*head_dim]")
+        check(lib().krb_qk_norm_rope_paged(
+            cache.ref, layer, qkv.data_ptr(), _pitch(qkv), out.data_ptr(), _pitch(out),
+            positions.data_ptr(), slots.data_ptr(), N, HQ, cos.data_ptr(), sin.data_ptr(),
+            cos.shape[0], _addr(q_norm), _addr(k_norm), eps, _addr(status), _stream(stream)), what)
+    return out
+
+
+def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=None, layer=0,
+                    out=None, workspace=None, status=None, stream=None):
+    """Attention of each sequence's new tokens (rows q_starts[b]:q_starts[b+1] of q [N, HQ*D],
+    already appended) over its cached positions: all kv_lens[b] - T_b positions before them and,
+    of the new ones, those up to itself (mask None) or those of its mask bits (int32 [N, words],
+    bit j % 32 of word j / 32 for new token j; a tree of drafted tokens).  page_table int32
+    [B, max_pages], kv_lens int32 [B], q_starts int32 [B+1], all on the device; max_q: no less
+    than any T_b.  workspace: a uint8 tensor of cache.attention_workspace(HQ, max_q) bytes that no
+    other call uses until this one is done (default: allocated per call)."""
+    import torch
+    what = "attention_paged"
+    dev, i32 = cache.device, torch.int32
+    _want(what, "q", q, cache.dtype, dev, 2)
+    N, width = q.shape
+    HQ = width // cache.head_dim
+    if HQ * cache.head_dim != width:
+        raise KrbError(f"{what}: q rows must hold HQ * head_dim values")
+    _want(what, "page_table", page_table, i32, dev, 2)
+    _want(what, "kv_lens", kv_lens, i32, dev, 1)
+    _want(what, "q_starts", q_starts, i32, dev, 1)
+    B = kv_lens.shape[0]
+    if page_table.shape[0] != B or q_starts.shape[0] != B + 1:
+        raise KrbError(f"{what}: page_table, kv_lens and q_starts must be of the same batch")
+    words = 0
+    if mask is not None:
+        _want(what, "mask", mask, i32, dev, 2)
+        if mask.shape[0] != N:
+            raise KrbError(f"{what}: mask must have one row per row of q")
+        words = mask.shape[1]
+    if status is not None:
+        _want(what, "status", status, i32, dev, 1)
+    need = cache.attention_workspace(HQ, max_q)
+    with _on(dev):
+        if out is None:
+            out = _empty((N, width), cache.dtype, dev, stream)
+        else:
+            _want(what, "out", out, cache.dtype, dev, 2)
+            if out.shape != q.shape:
+                raise KrbError(f"{what}: out must have q's shape")
+        if workspace is None:
+            workspace = _empty((need,), torch.uint8, dev, stream)
+        else:
+            _want(what, "workspace", workspace, torch.uint8, dev, 1)
+        check(lib().krb_attention_paged(
+            cache.ref, layer, q.data_ptr(), _pitch(q), out.data_ptr(), _pitch(out), N, HQ,
+            page_table.data_ptr(), _pitch(page_table), page_table.shape[1], kv_lens.data_ptr(),
+            q_starts.data_ptr(), B, max_q, _addr(mask), _pitch(mask) if words else 0, words, scale,
+            workspace.data_ptr(), workspace.numel(), _addr(status), _stream(stream)), what)
+    return out
+
+
+def kv_copy_pages(cache, src, dst, stream=None):
+    """Copy page src[i] to page dst[i], K and V of all layers (a fork's page of its own, or pages
+    moved together).  src, dst: host sequences of page numbers; no page is written twice, or both
+    read and written."""
+    n = len(src)
+    if len(dst) != n:
+        raise KrbError("kv_copy_pages: src and dst differ in length")
+    try:
+        pages = (c_int * (2 * n))(*src, *dst)
+    except TypeError as e:
+        raise KrbError(f"kv_copy_pages: src and dst must be host integers ({e})") from None
+    at = ctypes.addressof(pages)
+    with _on(cache.device):
+        check(lib().krb_kv_copy_pages(cache.ref, at, at + 4 * n, n, _stream(stream)),
+              "kv_copy_pages")
+
+
+def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=None):
+    """Keep the accepted tokens of verified drafts: K and V of position bases[b] + accepted[b][i]
+    move to position bases[b] + i for i < counts[b], all layers.  accepted int32 [B, A], ascending
+    strictly from >= 0 per sequence; bases, counts int32 [B]; page_table as in attention_paged."""
+    import torch
+    what = "kv_commit"
+    dev, i32 = cache.device, torch.int32
+    _want(what, "page_table", page_table, i32, dev, 2)
+    _want(what, "accepted", accepted, i32, dev, 2)
+    _want(what, "bases", bases, i32, dev, 1)
+    _want(what, "counts", counts, i32, dev, 1)
+    B, A = accepted.shape
+    if page_table.shape[0] != B or bases.shape[0] != B or counts.shape[0] != B:
+        raise KrbError(f"{what}: page_table, bases, accepted and counts must be of the same batch")
+    if status is not None:
+        _want(what, "status", status, i32, dev, 1)
+    with _on(dev):
+        check(lib().krb_kv_commit(
+            cache.ref, page_table.data_ptr(), _pitch(page_table), page_table.shape[1],
+            bases.data_ptr(), accepted.data_ptr(), _pitch(accepted), A, counts.data_ptr(), B,
+            _addr(status), _stream(stream)), what)
 
 
 def relay_down_single(act, w_down, resid, gamma, tiles, eps, bn=0, status=None, stream=None):

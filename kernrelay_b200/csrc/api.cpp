@@ -22,6 +22,7 @@
 #include "kernrelay.h"
 #include "kernrelay_b200.h"
 #include "model.h"
+#include "paged.h"
 #include "plan.h"
 #include "ptx.cuh"
 #include "synth.cuh"
@@ -617,6 +618,67 @@ KRB_EXPORT int krb_qk_norm_rope_bf16(void *qkv, int S, int HQ, int HKV, int D, c
   krb::qk_norm_rope_bf16(static_cast<bf *>(qkv), S, HQ, HKV, D, static_cast<const bf *>(cos_tab),
                          static_cast<const bf *>(sin_tab), static_cast<const bf *>(q_norm),
                          static_cast<const bf *>(k_norm), eps, as_stream(stream));
+  KRB_OP_END
+}
+
+KRB_EXPORT int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv,
+                                      int64_t ldqkv, void *q_out, int64_t ldq,
+                                      const int64_t *positions, const int64_t *slots, int N, int HQ,
+                                      const void *cos_tab, const void *sin_tab, int max_pos,
+                                      const void *q_norm, const void *k_norm, float eps,
+                                      uint32_t *status, void *stream) {
+  KRB_OP_BEGIN
+  krb::check_cache(cache, layer, "qk_norm_rope_paged");
+  krb::qk_norm_rope_paged(*cache, layer, qkv, ldqkv, q_out, ldq, positions, slots, N, HQ,
+                          static_cast<const bf *>(cos_tab), static_cast<const bf *>(sin_tab),
+                          max_pos, static_cast<const bf *>(q_norm), static_cast<const bf *>(k_norm),
+                          eps, status, as_stream(stream));
+  KRB_OP_END
+}
+
+KRB_EXPORT int krb_attention_paged(const krb_kv_cache *cache, int layer, const void *q, int64_t ldq,
+                                   void *out, int64_t ldo, int N, int HQ,
+                                   const int32_t *page_table, int64_t ldp, int max_pages,
+                                   const int32_t *kv_lens, const int32_t *q_starts, int B,
+                                   int max_q, const uint32_t *mask, int64_t ldm, int mask_words,
+                                   float scale, void *workspace, size_t workspace_bytes,
+                                   uint32_t *status, void *stream) {
+  KRB_OP_BEGIN
+  krb::check_cache(cache, layer, "attention_paged");
+  krb::attention_paged(*cache, layer,
+                       {q, long(ldq), out, long(ldo), N, HQ, page_table, long(ldp), max_pages,
+                        kv_lens, q_starts, B, max_q, mask, long(ldm), mask_words, scale, workspace,
+                        workspace_bytes, status},
+                       as_stream(stream));
+  KRB_OP_END
+}
+
+KRB_EXPORT size_t krb_attention_paged_workspace(const krb_kv_cache *cache, int HQ, int max_q) {
+  try {
+    krb::check_cache(cache, 0, "attention_paged");
+    return krb::attention_paged_workspace(*cache, HQ, max_q);
+  } catch (const std::exception &e) {
+    fail(e);
+    return 0;
+  }
+}
+
+KRB_EXPORT int krb_kv_copy_pages(const krb_kv_cache *cache, const int32_t *src, const int32_t *dst,
+                                 int n, void *stream) {
+  KRB_OP_BEGIN
+  krb::check_cache(cache, 0, "kv_copy_pages");
+  krb::kv_copy_pages(*cache, src, dst, n, as_stream(stream));
+  KRB_OP_END
+}
+
+KRB_EXPORT int krb_kv_commit(const krb_kv_cache *cache, const int32_t *page_table, int64_t ldp,
+                             int max_pages, const int32_t *bases, const int32_t *accepted,
+                             int64_t lda, int A, const int32_t *counts, int B, uint32_t *status,
+                             void *stream) {
+  KRB_OP_BEGIN
+  krb::check_cache(cache, 0, "kv_commit");
+  krb::kv_commit(*cache, page_table, ldp, max_pages, bases, accepted, lda, A, counts, B, status,
+                 as_stream(stream));
   KRB_OP_END
 }
 

@@ -1,0 +1,612 @@
+// Attention of new tokens over the paged K/V cache: the form for few query rows (a token or a
+// small draft per sequence) on mma.sync, the kernel that joins split units, and the host side.
+//
+// Few rows are bound by reading K and V once: a 64-key block of one KV head is 32 KB at
+// head_dim 128 and feeds 4 * rows * 64 * 128 flop, 1 us of one SM's share of HBM bandwidth for
+// 0.13 us of tensor work at 16 rows.  So the kernel is a deep ring of TMA loads (two CTAs of three
+// 32 KB stages per SM, about twice the bytes that latency needs in flight) and the rows of all
+// query heads that share a KV head go through the tensor cores together.  mma.sync takes 16-row
+// tiles, so 7 rows of a decoded token cost one of them; tcgen05 would pad them to 64 or 128.
+#include <algorithm>
+#include <string>
+
+#include "attention_paged.cuh"
+
+namespace krb {
+namespace paged {
+
+namespace {
+
+constexpr int kKeys = 64;        // keys of a block
+constexpr int kThreads = 160;    // 4 consumer warps, 1 producer warp
+constexpr int kConsumers = 128;
+
+template <int D>
+struct Cfg {
+  static constexpr int kHalf = kKeys * 128;             // 64 keys x 64 elements, bytes
+  static constexpr int kTile = kKeys * D * 2;           // K or V block
+  static constexpr int kStages = D == 128 ? 3 : 6;      // 96 KB of ring
+  static constexpr int kMergeLane = D / 16 * 4 + 4;     // floats per lane: half of O, m and l
+  static constexpr int kMerge = kMergeLane * 32 * 4;    // bytes per sending warp
+  static constexpr int kBars = 2 * kStages * 8;
+  static constexpr int kSmem =
+      2 * kStages * kTile + 2 * kMerge + kBars + int(sizeof(WalkStart)) + 16 + 1024;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+        " {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+        " {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// byte offset of 16-byte chunk `chunk` of key row `key` in a block (128-byte swizzle)
+template <int D>
+__device__ __forceinline__ uint32_t tile_off(int key, int chunk) {
+  return (chunk >> 3) * Cfg<D>::kHalf + key * 128 + (((chunk & 7) ^ (key & 7)) << 4);
+}
+
+}  // namespace
+
+// Warp (wm, wn) of the WM x (4 / WM) consumer warps: rows 16 wm .. +15 of the unit, keys
+// wn * 16 WM .. of every block.  A lane holds rows g = lane / 4 and g + 8 (mma fragments).
+template <int D, int WM, bool F16>
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_paged_kernel(const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const Params p, int box_shift) {
+  using C = Cfg<D>;
+  constexpr int WN = 4 / WM;
+  constexpr int kWarpKeys = kKeys / WN;
+  constexpr int NT = kWarpKeys / 8;  // 8-key score tiles of a warp
+  constexpr int DT = D / 8;          // 8-column output tiles
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem =
+      reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float *merge = reinterpret_cast<float *>(smem + 2 * C::kStages * C::kTile);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + 2 * C::kStages * C::kTile + 2 * C::kMerge);
+  uint64_t *empty = full + C::kStages;
+  WalkStart *start = reinterpret_cast<WalkStart *>(empty + C::kStages);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    const WalkStart s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
+    if (lane == 0) *start = s;
+  }
+  __syncthreads();
+  Walk w = begin_walk<kKeys>(p, *start);
+
+  if (warp == 4) {
+    // ---------------- producer: one TMA box per lane (page x half x K or V)
+    constexpr int kKinds = D / 64 * 2;
+    const int box = 1 << box_shift;
+    const int bx = lane / kKinds, kind = lane % kKinds;
+    const bool is_v = kind >= D / 64;
+    const int half = kind % (D / 64);
+    const CUtensorMap *map = is_v ? &tm_v : &tm_k;
+    int n = 0;  // blocks issued
+    bool ok = true;
+    while (w.pos < w.end && ok) {
+      const int e = piece_end(w);
+      const int end = kv_end(p, w.T, w.ctx, w.i);
+      for (int blk = w.blk; blk < e; ++blk, ++n) {
+        const int s = n % C::kStages;
+        const int key = blk * kKeys + (bx << box_shift);
+        const int nbox = (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift;
+        const int page = bx < nbox ? page_of(p, w.b, key) : 0;
+        ok = mbar_wait(&empty[s], ((n / C::kStages) & 1) ^ 1, kMbarLimitNs);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        uint8_t *stage = smem + s * 2 * C::kTile;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], nbox * box * 128 * kKinds);
+        __syncwarp();
+        if (bx < nbox)
+          tma_load_4d(stage + (is_v ? C::kTile : 0) + half * C::kHalf + (bx << box_shift) * 128,
+                      map, &full[s], half * 64, key & ((1 << p.page_shift) - 1), w.h, page);
+      }
+      if (ok) next_unit<kKeys>(p, w, e);
+    }
+    if (!ok && lane == 0) report_status(p.status, kStatusTmaWait);
+    // no TMA write may still be in flight when the CTA exits
+    for (int i = max(0, n - C::kStages); i < n; ++i)
+      mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, kMbarLimitNs / 4);
+    return;
+  }
+
+  // ---------------- consumers
+  const int wm = warp % WM, wn = warp / WM;
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  const uint32_t base = smem_u32(smem);
+  int n = 0;
+  bool ok = true;
+  while (w.pos < w.end) {
+    const int e = piece_end(w);
+    const int end = kv_end(p, w.T, w.ctx, w.i);
+    const int tok0 = w.i * p.tpt;
+    const int nrows = min(p.tpt, w.T - tok0) * p.group;
+    // rows g and g + 8 of this warp's tile: token and head
+    int tok[2], hd[2];
+    bool row_ok[2];
+    uint32_t qf[D / 16][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = wm * 16 + g + 8 * x;
+      row_ok[x] = r < nrows;
+      tok[x] = tok0 + r / p.group;
+      hd[x] = w.h * p.group + r % p.group;
+      const uint16_t *q = p.q + (w.q0 + tok[x]) * p.ldq + static_cast<long>(hd[x]) * D + c2;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[ks][x] = row_ok[x] ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16)) : 0u;
+        qf[ks][2 + x] = row_ok[x] ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16 + 8)) : 0u;
+      }
+    }
+    float o[DT][4];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int blk = w.blk; blk < e; ++blk, ++n) {
+      const int s = n % C::kStages;
+      if (ok) ok = mbar_wait(&full[s], (n / C::kStages) & 1, kMbarLimitNs);
+      if (!__all_sync(0xffffffffu, ok)) {  // leave the waits, keep the CTA's barriers in step
+        ok = false;
+        continue;
+      }
+      const int k0 = blk * kKeys + wn * kWarpKeys;  // this warp's first key
+      const uint32_t kt = base + s * 2 * C::kTile, vt = kt + C::kTile;
+      const bool wrote = k0 + kWarpKeys > end;
+      if (wrote) {
+        // V rows behind the last key may be anything (stale or never written memory, whose
+        // infinities a zero probability would not cancel): zero them
+        const int z0 = max(k0, end) - blk * kKeys, z1 = (wn + 1) * kWarpKeys;
+        for (int u = lane; u < (z1 - z0) * (D / 8); u += 32) {
+          const int key = z0 + u / (D / 8);
+          const uint32_t at = vt + tile_off<D>(key, u % (D / 8));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+        }
+        __syncwarp();
+      }
+      if (k0 < end) {
+        float sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[t][x] = 0.f;
+        const int krow = wn * kWarpKeys + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+          for (int t = 0; t < NT; t += 2) {
+            uint32_t b[4];
+            ldsm4(kt + tile_off<D>(krow + t * 8, 2 * ks + ((lane >> 3) & 1)), b);
+            mma16816<F16>(sc[t], qf[ks], b[0], b[1]);
+            mma16816<F16>(sc[t + 1], qf[ks], b[2], b[3]);
+          }
+        // the first row's token decides whether anything of these keys is hidden
+        if (k0 + kWarpKeys > w.ctx + (p.mask ? 0 : tok0 + 1)) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t *row_mask =
+                p.mask ? p.mask + (w.q0 + (row_ok[x] ? tok[x] : tok0)) * p.ldm : nullptr;
+#pragma unroll
+            for (int k = 0; k < kWarpKeys; k += 32) {
+              const uint32_t see = visible32(p, row_mask, w.T, tok[x], k0 + k - w.ctx);
+#pragma unroll
+              for (int t = k / 8; t < NT && t < k / 8 + 4; ++t)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  if (!((see >> (t * 8 - k + c2 + y)) & 1)) sc[t][2 * x + y] = -INFINITY;
+            }
+          }
+        }
+        float mx[2] = {m[0], m[1]};
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          top[0] = fmaxf(top[0], fmaxf(sc[t][0], sc[t][1]));
+          top[1] = fmaxf(top[1], fmaxf(sc[t][2], sc[t][3]));
+        }
+        float off[2], alpha[2];
+        bool moved = false;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+          m[x] = fmaxf(m[x], top[x] * p.scale_log2);
+          // a row that has seen nothing yet has no maximum: any offset gives its zeros
+          off[x] = m[x] == -INFINITY ? 0.f : m[x];
+          alpha[x] = exp2_mufu(mx[x] - off[x]);
+          moved |= m[x] != mx[x];
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) l[x] *= alpha[x];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            o[d][0] *= alpha[0];
+            o[d][1] *= alpha[0];
+            o[d][2] *= alpha[1];
+            o[d][3] *= alpha[1];
+          }
+        }
+        // P enters the second product in the cache's type (its relative rounding, 2^-9 or 2^-12,
+        // is that of the output); the row sum takes the fp32 values
+        uint32_t pf[NT / 2][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float p0 = exp2_mufu(fmaf(sc[t][2 * x], p.scale_log2, -off[x]));
+            const float p1 = exp2_mufu(fmaf(sc[t][2 * x + 1], p.scale_log2, -off[x]));
+            l[x] += p0 + p1;
+            pf[t / 2][(t & 1) * 2 + x] = pack2<F16>(p0, p1);
+          }
+        }
+        const int vrow = wn * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+        for (int ks = 0; ks < NT / 2; ++ks)
+#pragma unroll
+          for (int d = 0; d < DT; d += 2) {
+            uint32_t b[4];
+            ldsm4_t(vt + tile_off<D>(vrow + ks * 16, d + (lane >> 4)), b);
+            mma16816<F16>(o[d], pf[ks], b[0], b[1]);
+            mma16816<F16>(o[d + 1], pf[ks], b[2], b[3]);
+          }
+      }
+      if (wrote) fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    }
+
+    if constexpr (WN > 1) {
+      // the warps that share rows join: O in two halves (one fragment register of all lanes side
+      // by side, so no bank conflicts), wn 2, 3 -> 0, 1, then 1 -> 0 (WN = 2: 1 -> 0)
+      float fa[2][2], fb[2][2];  // per step and row: factors of the own and of the received O
+      auto send = [&](float *buf, int h) {
+#pragma unroll
+        for (int d = 0; d < DT / 2; ++d)
+          reinterpret_cast<float4 *>(buf)[d * 32 + lane] =
+              make_float4(o[h * DT / 2 + d][0], o[h * DT / 2 + d][1], o[h * DT / 2 + d][2],
+                          o[h * DT / 2 + d][3]);
+        reinterpret_cast<float4 *>(buf)[DT / 2 * 32 + lane] = make_float4(m[0], m[1], l[0], l[1]);
+      };
+      auto take = [&](const float *buf, int h, int step) {
+        if (h == 0) {
+          const float4 v = reinterpret_cast<const float4 *>(buf)[DT / 2 * 32 + lane];
+          const float vm[2] = {v.x, v.y}, vl[2] = {v.z, v.w};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float mm = fmaxf(m[x], vm[x]);
+            const float off = mm == -INFINITY ? 0.f : mm;
+            fa[step][x] = exp2_mufu(m[x] - off);
+            fb[step][x] = exp2_mufu(vm[x] - off);
+            m[x] = mm;
+            l[x] = l[x] * fa[step][x] + vl[x] * fb[step][x];
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < DT / 2; ++d) {
+          const float4 v = reinterpret_cast<const float4 *>(buf)[d * 32 + lane];
+          float(&t)[4] = o[h * DT / 2 + d];
+          t[0] = t[0] * fa[step][0] + v.x * fb[step][0];
+          t[1] = t[1] * fa[step][0] + v.y * fb[step][0];
+          t[2] = t[2] * fa[step][1] + v.z * fb[step][1];
+          t[3] = t[3] * fa[step][1] + v.w * fb[step][1];
+        }
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float *buf = merge + (warp & 1) * (C::kMerge / 4);
+        float *buf1 = merge + C::kMerge / 4;
+        named_bar_sync(1, kConsumers);  // the buffers' last readers are done
+        if (warp >= 2) send(buf, h);
+        named_bar_sync(1, kConsumers);
+        if (warp < 2) take(buf, h, 0);
+        if constexpr (WN == 4) {
+          if (warp == 1) send(buf1, h);
+          named_bar_sync(1, kConsumers);
+          if (warp == 0) take(buf1, h, 1);
+        }
+      }
+    }
+
+    if (wn == 0 && ok) {
+      const bool whole = w.blk == 0 && e == w.nblk;
+      if (whole) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (!row_ok[x]) continue;
+          const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
+          uint16_t *out = p.out + (w.q0 + tok[x]) * p.ldo + static_cast<long>(hd[x]) * D + c2;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            *reinterpret_cast<uint32_t *>(out + d * 8) =
+                pack2<F16>(o[d][2 * x] * inv, o[d][2 * x + 1] * inv);
+        }
+      } else {
+        const int slot = w.blk == 0;
+        float *ml = slot_ml(p, blockIdx.x, slot);
+        float *po = slot_o(p, blockIdx.x, slot);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = wm * 16 + g + 8 * x;
+          if (!row_ok[x]) continue;
+          if ((lane & 3) == 0) {
+            ml[r] = m[x];
+            ml[p.rows + r] = l[x];
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            *reinterpret_cast<float2 *>(po + r * D + d * 8 + c2) =
+                make_float2(o[d][2 * x], o[d][2 * x + 1]);
+        }
+      }
+    }
+    const bool goes_on = w.blk == 0 && e < w.nblk;
+    if (threadIdx.x == 0 && goes_on) p.desc[blockIdx.x] = split_desc(p, w);
+    next_unit<kKeys>(p, w, e);
+    // the piece that goes on is this CTA's last
+    if (threadIdx.x == 0 && w.pos >= w.end && !goes_on) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
+  if (start->pos >= start->end && threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (!ok && lane == 0) report_status(p.status, kStatusEpiWait);
+}
+
+// ------------------------------------------------------------------ joining split units
+// CTA (c, y) joins rows y * 4 .. of the unit that CTA c of the attention kernel began and later
+// ones went on with: a warp per row, O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+  constexpr int V = D / 32;  // columns of a lane
+  pdl_wait();
+  const int c = blockIdx.x;
+  const int4 d = p.desc[c];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * 4 + warp;
+  if (d.w < 2 || r >= d.y * p.group) return;
+  const int tok = r / p.group, g = r - tok * p.group;
+  const int sr = slot_row(p, tok, g);
+  float mx = -INFINITY;
+  for (int k = lane; k < d.w; k += 32) mx = fmaxf(mx, slot_ml(p, c + k, k == 0)[sr]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float off = mx == -INFINITY ? 0.f : mx;
+  float total = 0.f, acc[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) acc[x] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < d.w; ++k) {
+    const float *ml = slot_ml(p, c + k, k == 0);
+    const float f = exp2_mufu(ml[sr] - off);
+    total += f * ml[p.rows + sr];
+    const float *o = slot_o(p, c + k, k == 0) + static_cast<long>(sr) * D + lane * V;
+    if constexpr (V == 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(o);
+      acc[0] += f * v.x;
+      acc[1] += f * v.y;
+      acc[2] += f * v.z;
+      acc[3] += f * v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2 *>(o);
+      acc[0] += f * v.x;
+      acc[1] += f * v.y;
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  uint16_t *out = p.out + (d.x + tok) * p.ldo + static_cast<long>(d.z * p.group + g) * D + lane * V;
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<F16>(acc[0] * inv, acc[1] * inv),
+                                                 pack2<F16>(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t *>(out) = pack2<F16>(acc[0] * inv, acc[1] * inv);
+}
+
+// ------------------------------------------------------------------ host side
+void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas, (p.tpt * p.group + 3) / 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, true> : combine_kernel<128, false>)
+                          : (f16 ? combine_kernel<64, true> : combine_kernel<64, false>);
+  KRB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys) {
+  KvMaps r;
+  r.box = std::min(c.page_size, keys);
+  const uint64_t dims[4] = {uint64_t(c.head_dim), uint64_t(c.page_size), uint64_t(c.heads),
+                            uint64_t(c.pages)};
+  auto make = [&](const void *mem, const int64_t *st) {
+    // an axis of length 1 is never stepped along: any legal stride will do
+    const uint64_t s[3] = {uint64_t(st[3]), c.heads > 1 ? uint64_t(st[2]) : 8,
+                           c.pages > 1 ? uint64_t(st[1]) : 8};
+    return make_tmap_4d_2byte(static_cast<const uint16_t *>(mem) + (c.layers > 1 ? layer * st[0] : 0),
+                              dims, s, r.box);
+  };
+  r.k = make(c.k, c.k_stride);
+  r.v = make(c.v, c.v_stride);
+  return r;
+}
+
+static size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+size_t workspace_bytes(int ctas, int rows, int D) {
+  return align256(ctas * sizeof(int4)) + align256(size_t(ctas) * 4 * rows * sizeof(float)) +
+         size_t(ctas) * 2 * rows * D * sizeof(float);
+}
+
+void carve_workspace(Params &p, int ctas, void *ws) {
+  uint8_t *b = static_cast<uint8_t *>(ws);
+  p.desc = reinterpret_cast<int4 *>(b);
+  b += align256(ctas * sizeof(int4));
+  p.ml = reinterpret_cast<float *>(b);
+  b += align256(size_t(ctas) * 4 * p.rows * sizeof(float));
+  p.o = reinterpret_cast<float *>(b);
+}
+
+template <int D, int WM, bool F16>
+static void launch(const Params &p, const KvMaps &maps, int ctas, int device, cudaStream_t stream) {
+  auto *kern = attn_paged_kernel<D, WM, F16>;
+  static bool configured[64] = {false};
+  if (!configured[device & 63]) {
+    KRB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+    configured[device & 63] = true;
+  }
+  int box_shift = 0;
+  while ((1 << box_shift) < maps.box) ++box_shift;
+  kern<<<ctas, kThreads, Cfg<D>::kSmem, stream>>>(maps.k, maps.v, p, box_shift);
+  KRB_CUDA(cudaGetLastError());
+}
+
+template <int D, bool F16>
+static void launch_wm(int wm, const Params &p, const KvMaps &maps, int ctas, int device,
+                      cudaStream_t stream) {
+  if (wm == 1) launch<D, 1, F16>(p, maps, ctas, device, stream);
+  else if (wm == 2) launch<D, 2, F16>(p, maps, ctas, device, stream);
+  else launch<D, 4, F16>(p, maps, ctas, device, stream);
+}
+
+// The kernel of a call: 16-row tiles side by side (WM) from the most rows that a unit can have.
+struct Plan {
+  int wm, rows, ctas;
+};
+static Plan plan_of(int group, int max_q, int device) {
+  const long rows = long(max_q) * group;
+  Plan r;
+  r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  r.rows = 16 * r.wm;
+  r.ctas = 2 * sm_count(device);
+  return r;
+}
+
+static int group_of(const krb_kv_cache &c, int HQ, int max_q) {
+  if (HQ <= 0 || HQ % c.heads) throw CudaError("attention_paged: HQ must be a multiple of the cache's heads");
+  if (HQ / c.heads > 64) throw CudaError("attention_paged: more than 64 query heads per KV head");
+  if (max_q <= 0 || max_q > (1 << 24)) throw CudaError("attention_paged: bad max_q");
+  return HQ / c.heads;
+}
+
+}  // namespace paged
+
+size_t attention_paged_workspace(const krb_kv_cache &c, int HQ, int max_q) {
+  const int group = paged::group_of(c, HQ, max_q);
+  int device = 0;
+  KRB_CUDA(cudaGetDevice(&device));
+  const paged::Plan pl = paged::plan_of(group, max_q, device);
+  return paged::workspace_bytes(pl.ctas, pl.rows, c.head_dim);
+}
+
+void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, cudaStream_t stream) {
+  using namespace paged;
+  if (a.N < 0 || a.B < 0) throw CudaError("attention_paged: negative size");
+  const int group = group_of(c, a.HQ, a.max_q);
+  if (a.N == 0 || a.B == 0) return;
+  if (!a.q || !a.out || !a.page_table || !a.kv_lens || !a.q_starts)
+    throw CudaError("attention_paged: null pointer");
+  const long width = static_cast<long>(a.HQ) * c.head_dim;
+  if (a.ldq < width || a.ldo < width || a.ldq % 8 || a.ldo % 8)
+    throw CudaError("attention_paged: row pitch too small or not a multiple of 8");
+  for (const void *p : {a.q, static_cast<const void *>(a.out),
+                        static_cast<const void *>(a.workspace)})
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      throw CudaError("attention_paged: pointers must be 16-byte aligned");
+  if (a.max_pages <= 0 || a.ldp < a.max_pages)
+    throw CudaError("attention_paged: page table narrower than its rows");
+  if (int64_t(a.max_pages) * c.page_size > (int64_t(1) << 30))
+    throw CudaError("attention_paged: max_pages * page_size above 2^30");
+  if (!(a.scale > 0.f) || a.scale > 1e30f) throw CudaError("attention_paged: scale must be positive");
+  if (a.mask && (a.mask_words <= 0 || a.ldm < a.mask_words || long(a.mask_words) * 32 < a.max_q))
+    throw CudaError("attention_paged: mask rows narrower than max_q");
+  int device = 0;
+  KRB_CUDA(cudaGetDevice(&device));
+  const Plan pl = plan_of(group, a.max_q, device);
+  if (!a.workspace || a.workspace_bytes < workspace_bytes(pl.ctas, pl.rows, c.head_dim))
+    throw CudaError("attention_paged: workspace too small");
+
+  Params p{};
+  p.q = static_cast<const uint16_t *>(a.q);
+  p.out = static_cast<uint16_t *>(a.out);
+  p.ldq = a.ldq;
+  p.ldo = a.ldo;
+  p.page_table = a.page_table;
+  p.kv_lens = a.kv_lens;
+  p.q_starts = a.q_starts;
+  p.mask = a.mask;
+  p.ldp = a.ldp;
+  p.ldm = a.ldm;
+  p.N = a.N;
+  p.HQ = a.HQ;
+  p.HKV = c.heads;
+  p.group = group;
+  p.D = c.head_dim;
+  p.B = a.B;
+  p.max_q = a.max_q;
+  p.max_pages = a.max_pages;
+  p.pages = c.pages;
+  while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
+  p.mask_words = a.mask_words;
+  p.rows = pl.rows;
+  p.tpt = p.tile_tok = pl.rows / group;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = a.status;
+  carve_workspace(p, pl.ctas, a.workspace);
+
+  const bool f16 = c.dtype == 1;
+  const KvMaps maps = make_kv_maps(c, layer, kKeys);
+  if (p.D == 128 && f16) launch_wm<128, true>(pl.wm, p, maps, pl.ctas, device, stream);
+  else if (p.D == 128) launch_wm<128, false>(pl.wm, p, maps, pl.ctas, device, stream);
+  else if (f16) launch_wm<64, true>(pl.wm, p, maps, pl.ctas, device, stream);
+  else launch_wm<64, false>(pl.wm, p, maps, pl.ctas, device, stream);
+  launch_combine(p, pl.ctas, f16, stream);
+}
+
+}  // namespace krb

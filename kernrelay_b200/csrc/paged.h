@@ -1,0 +1,46 @@
+// The paged K/V cache as the kernels see it, and the launchers of its operators.
+#pragma once
+
+#include "common.h"
+#include "kernrelay_b200.h"
+
+namespace krb {
+
+// Throws on a cache the operators do not take (null pointers, sizes, alignment, strides whose
+// rows overlap); `layer` in [0, layers).
+void check_cache(const krb_kv_cache *c, int layer, const char *what);
+
+struct PagedAttnArgs {
+  const void *q;
+  long ldq;
+  void *out;
+  long ldo;
+  int N, HQ;
+  const int32_t *page_table;
+  long ldp;
+  int max_pages;
+  const int32_t *kv_lens, *q_starts;
+  int B, max_q;
+  const uint32_t *mask;
+  long ldm;
+  int mask_words;
+  float scale;
+  void *workspace;
+  size_t workspace_bytes;
+  uint32_t *status;
+};
+
+void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long ldqkv, void *q_out,
+                        long ldq, const int64_t *positions, const int64_t *slots, int N, int HQ,
+                        const __nv_bfloat16 *cos_tab, const __nv_bfloat16 *sin_tab, int max_pos,
+                        const __nv_bfloat16 *q_norm, const __nv_bfloat16 *k_norm, float eps,
+                        uint32_t *status, cudaStream_t stream);
+size_t attention_paged_workspace(const krb_kv_cache &c, int HQ, int max_q);
+void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, cudaStream_t stream);
+void kv_copy_pages(const krb_kv_cache &c, const int32_t *src, const int32_t *dst, int n,
+                   cudaStream_t stream);
+void kv_commit(const krb_kv_cache &c, const int32_t *page_table, long ldp, int max_pages,
+               const int32_t *bases, const int32_t *accepted, long lda, int A,
+               const int32_t *counts, int B, uint32_t *status, cudaStream_t stream);
+
+}  // namespace krb

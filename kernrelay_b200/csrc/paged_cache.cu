@@ -1,0 +1,464 @@
+// Operators that write the paged K/V cache: append (with the per-head norms and the rotation),
+// page copies and the commit of a draft's accepted tokens.  All three move bytes: every kernel
+// here is bound by HBM bandwidth at size and by its launch when small.
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "paged.h"
+#include "ptx.cuh"
+
+namespace krb {
+
+// ------------------------------------------------------------------ arguments
+static void check_strides(const int64_t *st, const krb_kv_cache &c, const std::string &what) {
+  const int64_t n[4] = {c.layers, c.pages, c.heads, c.page_size};
+  int order[4] = {0, 1, 2, 3};
+  std::sort(order, order + 4, [&](int a, int b) { return st[a] < st[b]; });
+  int64_t span = c.head_dim;  // extent of the axes with smaller strides, in elements
+  for (int i : order) {
+    if (n[i] == 1) continue;  // never stepped along
+    if (st[i] % 8) throw CudaError(what + ": cache strides must be multiples of 8 elements");
+    if (st[i] < span) throw CudaError(what + ": cache strides overlap");
+    if (st[i] > (int64_t(1) << 38)) throw CudaError(what + ": cache stride too large");
+    span = st[i] * (n[i] - 1) + span;
+  }
+}
+
+void check_cache(const krb_kv_cache *c, int layer, const char *name) {
+  const std::string what(name);
+  if (!c) throw CudaError(what + ": no cache");
+  if (!c->k || !c->v) throw CudaError(what + ": cache without K or V");
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
+    throw CudaError(what + ": K and V must be 16-byte aligned");
+  if (c->dtype != 0 && c->dtype != 1) throw CudaError(what + ": cache dtype must be bf16 or fp16");
+  if (c->layers <= 0 || c->pages <= 0 || c->heads <= 0)
+    throw CudaError(what + ": cache without layers, pages or heads");
+  if (c->head_dim != 64 && c->head_dim != 128) throw CudaError(what + ": head_dim must be 64 or 128");
+  if (c->page_size < 8 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)))
+    throw CudaError(what + ": page_size must be a power of two from 8 on");
+  if (layer < 0 || layer >= c->layers) throw CudaError(what + ": no such layer");
+  check_strides(c->k_stride, *c, what);
+  check_strides(c->v_stride, *c, what);
+}
+
+namespace {
+
+int ilog2(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+// ------------------------------------------------------------------ append
+struct AppendArgs {
+  const uint16_t *qkv;
+  long ldqkv;
+  uint16_t *q_out;
+  long ldq;
+  uint16_t *k, *v;                               // this layer
+  long k_page, k_head, k_slot, v_page, v_head, v_slot;  // strides in elements
+  const int64_t *positions, *slots;
+  const __nv_bfloat16 *cos_tab, *sin_tab, *q_norm, *k_norm;
+  int N, HQ, HKV, max_pos, page_shift;
+  int64_t total_slots;
+  float eps;
+  uint32_t *status;
+};
+
+template <bool F16>
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&f)[8]) {
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 t = unpack2<F16>(ws[e]);
+    f[2 * e] = t.x;
+    f[2 * e + 1] = t.y;
+  }
+}
+
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint4 w;
+  w.x = pack2<F16>(f[0], f[1]);
+  w.y = pack2<F16>(f[2], f[3]);
+  w.z = pack2<F16>(f[4], f[5]);
+  w.w = pack2<F16>(f[6], f[7]);
+  return w;
+}
+
+__device__ __forceinline__ uint4 ldg4(const void *p) {
+  return __ldg(reinterpret_cast<const uint4 *>(p));
+}
+
+// One thread = 8 rotation pairs (elements j..j+7 and D/2+j..D/2+j+7) of one head of one token;
+// the D/16 threads of a head are neighbours in a warp and share its sum of squares.
+//   x^ = x * rsqrt(mean(x^2) + eps) * w;  y_lo = x_lo cos_lo - x_hi sin_lo,
+//   y_hi = x_hi cos_hi + x_lo sin_hi
+// in fp32 from the stored values to the one rounding of the store.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+  constexpr int HALF = D / 2;
+  constexpr int kLanes = HALF / 8;
+  const long gt = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int nh = a.HQ + 2 * a.HKV;
+  const long item = gt / kLanes;
+  const int j = static_cast<int>(gt % kLanes) * 8;
+  if (item >= static_cast<long>(a.N) * nh) return;  // whole heads only
+  const int n = static_cast<int>(item / nh);
+  const int h = static_cast<int>(item - static_cast<long>(n) * nh);
+  const uint16_t *p = a.qkv + n * a.ldqkv + static_cast<long>(h) * D + j;
+  // plain loads: q_out may be the q columns of qkv
+  const uint4 wlo = *reinterpret_cast<const uint4 *>(p);
+  const uint4 whi = *reinterpret_cast<const uint4 *>(p + HALF);
+  const int64_t pos = a.positions[n];
+  const bool pos_ok = pos >= 0 && pos < a.max_pos;
+  if (!pos_ok && h == 0 && j == 0) report_status(a.status, kStatusBadIndex);
+
+  uint16_t *dst;
+  if (h < a.HQ) {
+    dst = a.q_out + n * a.ldq + static_cast<long>(h) * D + j;
+  } else {
+    const int64_t slot = a.slots[n];
+    const bool slot_ok = slot >= 0 && slot < a.total_slots;
+    if (!slot_ok && slot != -1 && h == a.HQ && j == 0) report_status(a.status, kStatusBadIndex);
+    // the D/16 threads of this head leave together (n and h are theirs alike)
+    if (!slot_ok || !pos_ok) return;
+    const long page = static_cast<long>(slot >> a.page_shift);
+    const long off = static_cast<long>(slot & ((int64_t(1) << a.page_shift) - 1));
+    if (h < a.HQ + a.HKV) {
+      dst = a.k + page * a.k_page + (h - a.HQ) * a.k_head + off * a.k_slot + j;
+    } else {
+      dst = a.v + page * a.v_page + (h - a.HQ - a.HKV) * a.v_head + off * a.v_slot + j;
+      *reinterpret_cast<uint4 *>(dst) = wlo;
+      *reinterpret_cast<uint4 *>(dst + HALF) = whi;
+      return;
+    }
+  }
+  if (!pos_ok) {
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4 *>(dst + HALF) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  float lo[8], hi[8];
+  unpack8<F16>(wlo, lo);
+  unpack8<F16>(whi, hi);
+  const __nv_bfloat16 *nw = h < a.HQ ? a.q_norm : a.k_norm;
+  if (nw) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+    const unsigned lane = threadIdx.x & 31;
+    const unsigned mask = ((1u << kLanes) - 1u) << (lane & ~unsigned(kLanes - 1));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    const float r = rsqrtf(ss * (1.0f / D) + a.eps);
+    float wl[8], wh[8];
+    unpack8<false>(ldg4(nw + j), wl);
+    unpack8<false>(ldg4(nw + HALF + j), wh);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] *= r * wl[e];
+      hi[e] *= r * wh[e];
+    }
+  }
+  const long t = pos * D + j;
+  float c[8], s[8], y[8];
+  unpack8<false>(ldg4(a.cos_tab + t), c);
+  unpack8<false>(ldg4(a.sin_tab + t), s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = lo[e] * c[e] - hi[e] * s[e];
+  *reinterpret_cast<uint4 *>(dst) = pack8<F16>(y);
+  unpack8<false>(ldg4(a.cos_tab + t + HALF), c);
+  unpack8<false>(ldg4(a.sin_tab + t + HALF), s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = hi[e] * c[e] + lo[e] * s[e];
+  *reinterpret_cast<uint4 *>(dst + HALF) = pack8<F16>(y);
+}
+
+// ------------------------------------------------------------------ page copies
+// Pages travel to the kernel in its parameters: the host arrays are read before the call
+// returns, and a captured launch keeps its own copy.
+constexpr int kPairsPerLaunch = 448;
+
+struct CopyArgs {
+  uint4 *base[2];           // K, V
+  long layer[2], page[2];   // strides in 16-byte units
+  long outer[2], inner[2];  // strides of the runs inside a page
+  int n_inner[2];           // runs per outer step
+  int run[2];               // 16-byte units per contiguous run
+  int units;                // 16-byte units of a page (all heads)
+  int layers;
+  int32_t src[kPairsPerLaunch], dst[kPairsPerLaunch];
+};
+
+constexpr int kCopyVec = 4;
+
+// grid (chunks of a page, pairs, layers * 2): 256 threads move kCopyVec units each
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+  const int kv = blockIdx.z & 1;
+  const int layer = blockIdx.z >> 1;
+  const long base = layer * a.layer[kv];
+  uint4 *const mem = a.base[kv];
+  const uint4 *src = mem + base + a.src[blockIdx.y] * a.page[kv];
+  uint4 *dst = mem + base + a.dst[blockIdx.y] * a.page[kv];
+  const int run = a.run[kv], ni = a.n_inner[kv];
+  uint4 w[kCopyVec];
+  long at[kCopyVec];
+#pragma unroll
+  for (int i = 0; i < kCopyVec; ++i) {
+    const int u = (blockIdx.x * kCopyVec + i) * 256 + threadIdx.x;
+    const int r = u / run;
+    at[i] = u < a.units ? (r / ni) * a.outer[kv] + (r % ni) * a.inner[kv] + (u - r * run) : -1;
+    if (at[i] >= 0) w[i] = src[at[i]];
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyVec; ++i)
+    if (at[i] >= 0) dst[at[i]] = w[i];
+}
+
+// ------------------------------------------------------------------ commit
+struct CommitArgs {
+  uint16_t *k, *v;
+  long k_layer, k_page, k_head, k_slot, v_layer, v_page, v_head, v_slot;
+  const int32_t *page_table, *bases, *accepted, *counts;
+  long ldp, lda;
+  int max_pages, pages, A, page_shift, layers, heads;
+  uint32_t *status;
+};
+
+// One CTA = one sequence and some of its (layer, K or V, head) rows.  It checks the sequence's
+// whole list first (so that a refused one is left whole), keeps the page and slot of source and
+// target in shared memory for kCommitChunk tokens at a time, and a thread moves one 16-byte
+// column: it reads the chunk's sources, then writes its targets.  accepted ascends strictly from
+// >= 0, so target i <= source i < later sources: no source is overwritten before it is read,
+// whatever the chunks.
+constexpr int kCommitThreads = 256;
+constexpr int kCommitChunk = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
+  constexpr int kLanes = D / 8;
+  __shared__ int s_bad;
+  const int b = blockIdx.x;
+  const int n = a.counts[b];
+  const int64_t base = a.bases[b];
+  const int64_t room = static_cast<int64_t>(a.max_pages) << a.page_shift;
+  const bool sizes_ok = n >= 0 && n <= a.A && base >= 0 && base <= room;
+  if (threadIdx.x == 0) s_bad = !sizes_ok;
+  __syncthreads();
+  const int32_t *acc = a.accepted + b * a.lda;
+  const int32_t *table = a.page_table + b * a.ldp;
+  auto page_ok = [&](int64_t p) {
+    const int32_t id = table[p >> a.page_shift];
+    return id >= 0 && id < a.pages;
+  };
+  if (sizes_ok) {
+    for (int i = threadIdx.x; i < n; i += kCommitThreads) {
+      const int64_t x = acc[i];
+      const int64_t before = i ? acc[i - 1] : -1;
+      if (x <= before || base + x >= room || !page_ok(base + x) || !page_ok(base + i)) s_bad = 1;
+    }
+  }
+  __syncthreads();
+  if (s_bad) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) report_status(a.status, kStatusBadIndex);
+    return;
+  }
+  const int rows = a.layers * 2 * a.heads;
+  const int row = blockIdx.y * (kCommitThreads / kLanes) + threadIdx.x / kLanes;
+  if (row >= rows) return;
+  const int col = (threadIdx.x % kLanes) * 8;
+  const int h = row % a.heads;
+  const int kv = (row / a.heads) & 1;
+  const int layer = row / (2 * a.heads);
+  uint16_t *mem = kv ? a.v + layer * a.v_layer + h * a.v_head : a.k + layer * a.k_layer + h * a.k_head;
+  const long ps = kv ? a.v_page : a.k_page, ss = kv ? a.v_slot : a.k_slot;
+  auto at = [&](int64_t p) {
+    const long page = table[p >> a.page_shift];
+    return reinterpret_cast<uint4 *>(mem + page * ps + (p & ((1 << a.page_shift) - 1)) * ss + col);
+  };
+  for (int i0 = 0; i0 < n; i0 += kCommitChunk) {
+    uint4 w[kCommitChunk];
+#pragma unroll
+    for (int i = 0; i < kCommitChunk; ++i)
+      if (i0 + i < n && acc[i0 + i] != i0 + i) w[i] = *at(base + acc[i0 + i]);
+#pragma unroll
+    for (int i = 0; i < kCommitChunk; ++i)
+      if (i0 + i < n && acc[i0 + i] != i0 + i) *at(base + i0 + i) = w[i];
+  }
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ host side
+void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long ldqkv, void *q_out,
+                        long ldq, const int64_t *positions, const int64_t *slots, int N, int HQ,
+                        const __nv_bfloat16 *cos_tab, const __nv_bfloat16 *sin_tab, int max_pos,
+                        const __nv_bfloat16 *q_norm, const __nv_bfloat16 *k_norm, float eps,
+                        uint32_t *status, cudaStream_t stream) {
+  const int D = c.head_dim;
+  const int nh = HQ + 2 * c.heads;
+  if (N < 0 || HQ <= 0) throw CudaError("qk_norm_rope_paged: bad N or HQ");
+  if (N == 0) return;
+  if (!qkv || !q_out || !positions || !slots || !cos_tab || !sin_tab)
+    throw CudaError("qk_norm_rope_paged: null pointer");
+  if (!q_norm != !k_norm) throw CudaError("qk_norm_rope_paged: q_norm and k_norm, or neither");
+  if (max_pos <= 0) throw CudaError("qk_norm_rope_paged: empty rope tables");
+  if (ldqkv < static_cast<long>(nh) * D || ldq < static_cast<long>(HQ) * D || ldqkv % 8 || ldq % 8)
+    throw CudaError("qk_norm_rope_paged: row pitch too small or not a multiple of 8");
+  for (const void *p : {qkv, static_cast<const void *>(q_out), static_cast<const void *>(cos_tab),
+                        static_cast<const void *>(sin_tab), static_cast<const void *>(q_norm),
+                        static_cast<const void *>(k_norm)})
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      throw CudaError("qk_norm_rope_paged: pointers must be 16-byte aligned");
+  AppendArgs a{};
+  a.qkv = static_cast<const uint16_t *>(qkv);
+  a.ldqkv = ldqkv;
+  a.q_out = static_cast<uint16_t *>(q_out);
+  a.ldq = ldq;
+  a.k = static_cast<uint16_t *>(c.k) + layer * c.k_stride[0];
+  a.v = static_cast<uint16_t *>(c.v) + layer * c.v_stride[0];
+  a.k_page = c.k_stride[1];
+  a.k_head = c.k_stride[2];
+  a.k_slot = c.k_stride[3];
+  a.v_page = c.v_stride[1];
+  a.v_head = c.v_stride[2];
+  a.v_slot = c.v_stride[3];
+  a.positions = positions;
+  a.slots = slots;
+  a.cos_tab = cos_tab;
+  a.sin_tab = sin_tab;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.N = N;
+  a.HQ = HQ;
+  a.HKV = c.heads;
+  a.max_pos = max_pos;
+  a.page_shift = ilog2(c.page_size);
+  a.total_slots = int64_t(c.pages) * c.page_size;
+  a.eps = eps;
+  a.status = status;
+  const long threads = static_cast<long>(N) * nh * (D / 16);
+  const long blocks = (threads + 255) / 256;
+  if (blocks > 0x7fffffffL) throw CudaError("qk_norm_rope_paged: too many tokens");
+  const unsigned g = static_cast<unsigned>(blocks);
+  if (D == 128 && c.dtype) append_kernel<128, true><<<g, 256, 0, stream>>>(a);
+  else if (D == 128) append_kernel<128, false><<<g, 256, 0, stream>>>(a);
+  else if (c.dtype) append_kernel<64, true><<<g, 256, 0, stream>>>(a);
+  else append_kernel<64, false><<<g, 256, 0, stream>>>(a);
+  KRB_CUDA(cudaGetLastError());
+}
+
+void kv_copy_pages(const krb_kv_cache &c, const int32_t *src, const int32_t *dst, int n,
+                   cudaStream_t stream) {
+  if (n < 0) throw CudaError("kv_copy_pages: negative count");
+  if (n == 0) return;
+  if (!src || !dst) throw CudaError("kv_copy_pages: null pointer");
+  std::vector<char> written(c.pages, 0);
+  for (int i = 0; i < n; ++i) {
+    for (const int32_t p : {src[i], dst[i]})
+      if (p < 0 || p >= c.pages) throw CudaError("kv_copy_pages: no page " + std::to_string(p));
+    if (src[i] == dst[i]) continue;
+    if (written[dst[i]])
+      throw CudaError("kv_copy_pages: page " + std::to_string(dst[i]) + " is written twice");
+    written[dst[i]] = 1;
+  }
+  for (int i = 0; i < n; ++i)
+    if (src[i] != dst[i] && written[src[i]])
+      throw CudaError("kv_copy_pages: page " + std::to_string(src[i]) + " is read and written");
+  CopyArgs a;
+  const int64_t *strides[2] = {c.k_stride, c.v_stride};
+  void *mem[2] = {c.k, c.v};
+  const long d = c.head_dim / 8;
+  a.units = static_cast<int>(d) * c.heads * c.page_size;
+  if (static_cast<long>(a.units) != d * c.heads * c.page_size || a.units > (1 << 30))
+    throw CudaError("kv_copy_pages: page too large");
+  a.layers = c.layers;
+  for (int kv = 0; kv < 2; ++kv) {
+    a.base[kv] = static_cast<uint4 *>(mem[kv]);
+    a.layer[kv] = strides[kv][0] / 8;
+    a.page[kv] = strides[kv][1] / 8;
+    const long head = strides[kv][2] / 8, slot = strides[kv][3] / 8;
+    // runs of contiguous units: the inner axis (the one of smaller stride) joins the run when its
+    // steps are dense, then the outer one when that is dense too
+    const bool slots_inner = c.heads == 1 || (c.page_size > 1 && slot < head);
+    const long in_stride = slots_inner ? slot : head, out_stride = slots_inner ? head : slot;
+    const int in_n = slots_inner ? c.page_size : c.heads, out_n = slots_inner ? c.heads : c.page_size;
+    a.run[kv] = static_cast<int>(d);
+    a.n_inner[kv] = in_n;
+    a.inner[kv] = in_stride;
+    a.outer[kv] = out_stride;
+    if (in_n == 1 || in_stride == d) {
+      a.run[kv] = static_cast<int>(d) * in_n;
+      a.n_inner[kv] = out_n;
+      a.inner[kv] = out_stride;
+      a.outer[kv] = 0;
+      if (out_n == 1 || out_stride == a.run[kv]) {
+        a.run[kv] = a.units;
+        a.n_inner[kv] = 1;
+        a.inner[kv] = 0;
+      }
+    }
+  }
+  if (c.layers > 32767) throw CudaError("kv_copy_pages: too many layers");
+  for (int i = 0; i < n;) {
+    int m = 0;
+    for (; i < n && m < kPairsPerLaunch; ++i) {
+      if (src[i] == dst[i]) continue;
+      a.src[m] = src[i];
+      a.dst[m++] = dst[i];
+    }
+    if (!m) break;
+    const dim3 grid((a.units + 256 * kCopyVec - 1) / (256 * kCopyVec), m, 2 * c.layers);
+    copy_pages_kernel<<<grid, 256, 0, stream>>>(a);
+    KRB_CUDA(cudaGetLastError());
+  }
+}
+
+void kv_commit(const krb_kv_cache &c, const int32_t *page_table, long ldp, int max_pages,
+               const int32_t *bases, const int32_t *accepted, long lda, int A,
+               const int32_t *counts, int B, uint32_t *status, cudaStream_t stream) {
+  if (B < 0 || A < 0) throw CudaError("kv_commit: negative size");
+  if (B == 0 || A == 0) return;
+  if (!page_table || !bases || !accepted || !counts) throw CudaError("kv_commit: null pointer");
+  if (max_pages <= 0 || ldp < max_pages || lda < A)
+    throw CudaError("kv_commit: page table or accepted list narrower than its rows");
+  if ((int64_t(max_pages) << ilog2(c.page_size)) > (int64_t(1) << 30))
+    throw CudaError("kv_commit: max_pages * page_size above 2^30");
+  CommitArgs a{};
+  a.k = static_cast<uint16_t *>(c.k);
+  a.v = static_cast<uint16_t *>(c.v);
+  a.k_layer = c.k_stride[0];
+  a.k_page = c.k_stride[1];
+  a.k_head = c.k_stride[2];
+  a.k_slot = c.k_stride[3];
+  a.v_layer = c.v_stride[0];
+  a.v_page = c.v_stride[1];
+  a.v_head = c.v_stride[2];
+  a.v_slot = c.v_stride[3];
+  a.page_table = page_table;
+  a.bases = bases;
+  a.accepted = accepted;
+  a.counts = counts;
+  a.ldp = ldp;
+  a.lda = lda;
+  a.max_pages = max_pages;
+  a.pages = c.pages;
+  a.A = A;
+  a.page_shift = ilog2(c.page_size);
+  a.layers = c.layers;
+  a.heads = c.heads;
+  a.status = status;
+  const long rows = 2L * c.layers * c.heads;
+  const int per = kCommitThreads / (c.head_dim / 8);
+  const long gy = (rows + per - 1) / per;
+  if (gy > 65535) throw CudaError("kv_commit: too many layers and heads");
+  const dim3 grid(B, static_cast<unsigned>(gy));
+  if (c.head_dim == 128) commit_kernel<128><<<grid, kCommitThreads, 0, stream>>>(a);
+  else commit_kernel<64><<<grid, kCommitThreads, 0, stream>>>(a);
+  KRB_CUDA(cudaGetLastError());
+}
+
+}  // namespace krb

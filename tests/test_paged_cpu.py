@@ -1,0 +1,204 @@
+"""Refusals of the paged K/V cache operators, none of which reaches a GPU: through the C ABI with
+addresses that are never followed, and through the Python wrappers with CPU tensors."""
+import ctypes
+
+import pytest
+
+
+def _desc(krlib, **over):
+    d = krlib.KVCacheDesc(4096, 8192, 0, 2, 10, 4, 16, 128,
+                          (ctypes.c_int64 * 4)(81920, 8192, 2048, 128),
+                          (ctypes.c_int64 * 4)(81920, 8192, 2048, 128))
+    for key, x in over.items():
+        setattr(d, key, (ctypes.c_int64 * 4)(*x) if key.endswith("stride") else x)
+    return d
+
+
+def _message(krlib):
+    return krlib.lib().krb_last_error().decode()
+
+
+BAD_CACHES = [
+    (dict(k=0), "without K or V"), (dict(v=0), "without K or V"), (dict(k=4104), "aligned"),
+    (dict(dtype=2), "dtype"), (dict(layers=0), "layers"), (dict(pages=-1), "pages"),
+    (dict(heads=0), "heads"), (dict(head_dim=96), "head_dim"), (dict(page_size=24), "power of two"),
+    (dict(page_size=4), "power of two"),
+    (dict(k_stride=(81920, 8192, 2048, 120)), "overlap"),
+    (dict(v_stride=(81920, 8192, 2044, 128)), "multiples of 8"),
+    (dict(k_stride=(0, 8192, 2048, 128)), "overlap"),
+    (dict(v_stride=(81920, -8192, 2048, 128)), "overlap"),
+    (dict(k_stride=(40960, 8192, 2048, 128)), "overlap"),
+]
+
+
+@pytest.mark.parametrize("over,what", BAD_CACHES)
+def test_bad_caches(krlib, over, what):
+    L = krlib.lib()
+    ref = ctypes.addressof(d := _desc(krlib, **over))
+    one = (ctypes.c_int * 1)(1)
+    assert L.krb_kv_copy_pages(ref, one, one, 1, None) == 1 and what in _message(krlib)
+    assert L.krb_qk_norm_rope_paged(ref, 0, 16, 4096, 16, 4096, 16, 16, 1, 28, 16, 16, 8, None, None,
+                                    1e-6, None, None) == 1 and what in _message(krlib)
+    assert L.krb_attention_paged(ref, 0, 16, 3584, 16, 3584, 1, 28, 16, 8, 8, 16, 16, 1, 1, None, 0, 0,
+                                 0.1, 16, 1 << 30, None, None) == 1 and what in _message(krlib)
+    assert L.krb_kv_commit(ref, 16, 8, 8, 16, 16, 4, 4, 16, 1, None, None) == 1 and what in _message(krlib)
+    assert L.krb_attention_paged_workspace(ref, 28, 1) == 0 and what in _message(krlib)
+    del d
+    assert L.krb_kv_copy_pages(None, one, one, 1, None) == 1 and "no cache" in _message(krlib)
+
+
+def test_legal_cache_layouts(krlib):
+    """Axis orders and lengths of one that check_cache takes: the next refusal is reached."""
+    L = krlib.lib()
+    bad = (ctypes.c_int * 1)(99)
+    for over in (dict(), dict(k_stride=(81920, 8192, 128, 512), v_stride=(81920, 8192, 128, 512)),
+                 dict(k_stride=(8192 * 2, 8192 * 4, 2048, 128)),
+                 dict(layers=1, k_stride=(0, 8192, 2048, 128)),
+                 dict(heads=1, k_stride=(81920, 8192, 3, 128))):
+        d = _desc(krlib, **over)
+        assert L.krb_kv_copy_pages(ctypes.addressof(d), bad, bad, 1, None) == 1
+        assert "no page 99" in _message(krlib)
+
+
+@pytest.mark.parametrize("src,dst,what", [
+    ([0], [10], "no page 10"), ([-1], [2], "no page -1"), ([0, 1], [2, 2], "page 2 is written twice"),
+    ([0, 1], [1, 2], "page 1 is read and written"), ([1, 0], [2, 1], "page 1 is read and written"),
+])
+def test_copy_refusals(krlib, src, dst, what):
+    d = _desc(krlib)
+    a, b = ((ctypes.c_int * len(x))(*x) for x in (src, dst))
+    L = krlib.lib()
+    assert L.krb_kv_copy_pages(ctypes.addressof(d), a, b, len(src), None) == 1
+    assert what in _message(krlib)
+    assert L.krb_kv_copy_pages(ctypes.addressof(d), None, b, 1, None) == 1
+    assert "null" in _message(krlib)
+    assert L.krb_kv_copy_pages(ctypes.addressof(d), a, b, -1, None) == 1
+    assert L.krb_kv_copy_pages(ctypes.addressof(d), a, b, 0, None) == 0
+    same = (ctypes.c_int * 2)(3, 4)  # pages onto themselves: nothing to launch
+    assert L.krb_kv_copy_pages(ctypes.addressof(d), same, same, 2, None) == 0
+
+
+APPEND = dict(layer=0, qkv=16, ldqkv=36 * 128, q=16, ldq=28 * 128, pos=16, slots=16, N=3, HQ=28, cos=16,
+              sin=16, max_pos=8, qn=None, kn=None)
+
+
+@pytest.mark.parametrize("over,what", [
+    (dict(layer=2), "layer"), (dict(layer=-1), "layer"), (dict(N=-1), "bad N"), (dict(HQ=0), "bad N"),
+    (dict(qkv=None), "null"), (dict(pos=None), "null"), (dict(slots=None), "null"), (dict(cos=None), "null"),
+    (dict(qn=16), "neither"), (dict(max_pos=0), "empty"), (dict(ldqkv=36 * 128 - 8), "pitch"),
+    (dict(ldq=28 * 128 + 4), "pitch"), (dict(qkv=8), "aligned"), (dict(q=24), "aligned"),
+    (dict(qn=16, kn=18), "aligned"),
+])
+def test_append_refusals(krlib, over, what):
+    d, a = _desc(krlib), {**APPEND, **over}
+    rc = krlib.lib().krb_qk_norm_rope_paged(
+        ctypes.addressof(d), a["layer"], a["qkv"], a["ldqkv"], a["q"], a["ldq"], a["pos"], a["slots"],
+        a["N"], a["HQ"], a["cos"], a["sin"], a["max_pos"], a["qn"], a["kn"], 1e-6, None, None)
+    assert rc == 1 and what in _message(krlib)
+
+
+ATTN = dict(layer=0, q=16, ldq=28 * 128, out=16, ldo=28 * 128, N=3, HQ=28, table=16, ldp=8, P=8, lens=16,
+            starts=16, B=2, max_q=1, mask=None, ldm=0, words=0, scale=0.1, ws=16)
+
+
+@pytest.mark.parametrize("over,what", [
+    (dict(layer=2), "layer"), (dict(HQ=27), "multiple"), (dict(HQ=0), "multiple"),
+    (dict(HQ=4 * 65, ldq=65 * 512, ldo=65 * 512), "64 query heads"), (dict(max_q=0), "max_q"),
+    (dict(N=-1), "negative"), (dict(B=-1), "negative"), (dict(q=None), "null"), (dict(out=None), "null"),
+    (dict(table=None), "null"), (dict(lens=None), "null"), (dict(starts=None), "null"),
+    (dict(ldq=28 * 128 - 8), "pitch"), (dict(ldo=28 * 128 + 1), "pitch"), (dict(q=2), "aligned"),
+    (dict(out=8), "aligned"), (dict(ws=8), "aligned"), (dict(P=0), "page table"), (dict(ldp=7), "page table"),
+    (dict(P=1 << 27, ldp=1 << 27), "2^30"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(mask=16, words=0, ldm=4), "mask"), (dict(mask=16, words=1, ldm=1, max_q=33), "mask"),
+    (dict(mask=16, words=2, ldm=1), "mask"),
+])
+def test_attention_refusals(krlib, over, what):
+    d, a = _desc(krlib), {**ATTN, **over}
+    rc = krlib.lib().krb_attention_paged(
+        ctypes.addressof(d), a["layer"], a["q"], a["ldq"], a["out"], a["ldo"], a["N"], a["HQ"],
+        a["table"], a["ldp"], a["P"], a["lens"], a["starts"], a["B"], a["max_q"], a["mask"], a["ldm"],
+        a["words"], a["scale"], a["ws"], 1 << 40, None, None)
+    assert rc == 1 and what in _message(krlib)
+
+
+@pytest.mark.parametrize("over,what", [
+    (dict(table=None), "null"), (dict(bases=None), "null"), (dict(acc=None), "null"),
+    (dict(counts=None), "null"), (dict(P=0), "page table"), (dict(ldp=7), "page table"),
+    (dict(lda=3), "accepted"), (dict(B=-1), "negative"), (dict(A=-1), "negative"),
+    (dict(P=1 << 27, ldp=1 << 27), "2^30"),
+])
+def test_commit_refusals(krlib, over, what):
+    a = {**dict(table=16, ldp=8, P=8, bases=16, acc=16, lda=4, A=4, counts=16, B=2), **over}
+    d = _desc(krlib)
+    rc = krlib.lib().krb_kv_commit(ctypes.addressof(d), a["table"], a["ldp"], a["P"], a["bases"],
+                                   a["acc"], a["lda"], a["A"], a["counts"], a["B"], None, None)
+    assert rc == 1 and what in _message(krlib)
+
+
+def test_empty_calls_do_nothing(krlib):
+    d = ctypes.addressof(keep := _desc(krlib))
+    L = krlib.lib()
+    assert L.krb_qk_norm_rope_paged(d, 0, None, 0, None, 0, None, None, 0, 28, None, None, 0, None, None,
+                                    1e-6, None, None) == 0
+    for N, B in ((0, 2), (3, 0)):
+        assert L.krb_attention_paged(d, 0, None, 0, None, 0, N, 28, None, 0, 0, None, None, B, 1, None, 0,
+                                     0, 0.1, None, 0, None, None) == 0
+    for A, B in ((0, 2), (3, 0)):
+        assert L.krb_kv_commit(d, None, 0, 0, None, None, 0, A, None, B, None, None) == 0
+    del keep
+
+
+# ---------------------------------------------------------------- the wrappers
+def _cpu_cache(krlib, **kw):
+    import torch
+    k = torch.zeros(2, 6, 2, 16, 64, dtype=kw.get("dtype", torch.bfloat16))
+    return krlib.KVCache(k, torch.zeros_like(k))
+
+
+def test_cache_handle_refusals(krlib):
+    import torch
+    k = torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16)
+    c = krlib.KVCache(k, k.clone())
+    assert (c.layers, c.pages, c.heads, c.page_size, c.head_dim) == (1, 6, 2, 16, 64)
+    for a, b, what in ((k, k[:5], "must be"), (k[0], k[0], "must be"), (k.float(), k.float(), "bf16"),
+                       (k, k.half(), "bf16"), (k.transpose(2, 3), k.transpose(2, 3), "contiguous")):
+        with pytest.raises(krlib.KrbError, match=what):
+            krlib.KVCache(a, b)
+
+
+def test_wrapper_refusals(krlib):
+    import torch
+    c = _cpu_cache(krlib)
+    bf = torch.bfloat16
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    qkv, pos = torch.zeros(3, 8 * 64, dtype=bf), torch.zeros(3, dtype=torch.int64)
+    tab = torch.zeros(9, 64, dtype=bf)
+    good = dict(qkv=qkv, positions=pos, slots=pos, HQ=4, cos=tab, sin=tab)
+    for over, what in ((dict(qkv=qkv.half()), "qkv"), (dict(qkv=qkv[:, :-64]), "HKV"),
+                       (dict(positions=pos.int()), "positions"), (dict(slots=pos[:2]), "slots"),
+                       (dict(cos=tab.float()), "cos"), (dict(sin=tab[:5]), "cos and sin"),
+                       (dict(cos=tab[:, :32], sin=tab[:, :32]), "cos and sin"),
+                       (dict(q_norm=tab[0][:32]), "q_norm"), (dict(out=qkv[:, :64]), "out"),
+                       (dict(status=pos), "status")):
+        with pytest.raises(krlib.KrbError, match=what):
+            krlib.qk_norm_rope_paged(**{**good, "cache": c, **over})
+    q = torch.zeros(3, 4 * 64, dtype=bf)
+    c._workspaces[4, 1] = 64  # asked of the device elsewhere
+    good = dict(q=q, page_table=i32(2, 4), kv_lens=i32(2), q_starts=i32(3), max_q=1, scale=0.1)
+    for over, what in ((dict(q=q.half()), "q must"), (dict(q=q[:, :-1]), "head_dim"),
+                       (dict(page_table=i32(2, 4).long()), "page_table"), (dict(q_starts=i32(2)), "batch"),
+                       (dict(page_table=i32(1, 4)), "batch"), (dict(mask=i32(2, 1)), "mask"),
+                       (dict(mask=i32(3, 1).long()), "mask"), (dict(out=q[:2]), "out"),
+                       (dict(workspace=i32(9)), "workspace")):
+        with pytest.raises(krlib.KrbError, match=what):
+            krlib.attention_paged(**{**good, "cache": c, **over})
+    good = dict(page_table=i32(2, 4), bases=i32(2), accepted=i32(2, 3), counts=i32(2))
+    for over, what in ((dict(bases=i32(3)), "batch"), (dict(counts=i32(2).long()), "counts"),
+                       (dict(accepted=i32(3, 3)), "batch"), (dict(page_table=i32(4)), "page_table")):
+        with pytest.raises(krlib.KrbError, match=what):
+            krlib.kv_commit(c, **{**good, **over})
+    with pytest.raises(krlib.KrbError, match="length"):
+        krlib.kv_copy_pages(c, [1, 2], [3])
+    with pytest.raises(krlib.KrbError, match="host integers"):
+        krlib.kv_copy_pages(c, [1.5], [3])
