@@ -515,16 +515,32 @@ static void launch_wm(int wm, const Params &p, const KvMaps &maps, int ctas, int
   else launch<D, 4, F16>(p, maps, ctas, device, stream);
 }
 
-// The kernel of a call: 16-row tiles side by side (WM) from the most rows that a unit can have.
+CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int tok, int heads) {
+  const uint64_t dims[4] = {uint64_t(D), uint64_t(HQ), uint64_t(N), 1};
+  const uint64_t strides[3] = {uint64_t(D), uint64_t(ldq), 8};
+  return make_tmap_4d_2byte(q, dims, strides, heads, tok);
+}
+
+// The kernel of a call, from the most rows that a unit can have: mma.sync on 16 wm rows, or
+// tcgen05 on nt tiles of 128.
 struct Plan {
-  int wm, rows, ctas;
+  int wm, nt, rows, ctas, tile_tok, tpt;
 };
 static Plan plan_of(int group, int max_q, int device) {
   const long rows = long(max_q) * group;
-  Plan r;
-  r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  r.rows = 16 * r.wm;
-  r.ctas = 2 * sm_count(device);
+  Plan r{};
+  if (rows <= 64) {
+    r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    r.rows = 16 * r.wm;
+    r.ctas = 2 * sm_count(device);
+    r.tpt = r.tile_tok = r.rows / group;
+  } else {
+    r.tile_tok = 128 / group;
+    r.nt = max_q > r.tile_tok ? 2 : 1;
+    r.rows = 128 * r.nt;
+    r.ctas = sm_count(device);
+    r.tpt = r.nt * r.tile_tok;
+  }
   return r;
 }
 
@@ -595,17 +611,22 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
   p.mask_words = a.mask_words;
   p.rows = pl.rows;
-  p.tpt = p.tile_tok = pl.rows / group;
+  p.tpt = pl.tpt;
+  p.tile_tok = pl.tile_tok;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = a.status;
   carve_workspace(p, pl.ctas, a.workspace);
 
   const bool f16 = c.dtype == 1;
-  const KvMaps maps = make_kv_maps(c, layer, kKeys);
-  if (p.D == 128 && f16) launch_wm<128, true>(pl.wm, p, maps, pl.ctas, device, stream);
-  else if (p.D == 128) launch_wm<128, false>(pl.wm, p, maps, pl.ctas, device, stream);
-  else if (f16) launch_wm<64, true>(pl.wm, p, maps, pl.ctas, device, stream);
-  else launch_wm<64, false>(pl.wm, p, maps, pl.ctas, device, stream);
+  if (pl.nt) {
+    launch_tc(c, layer, p, pl.ctas, device, stream);
+  } else {
+    const KvMaps maps = make_kv_maps(c, layer, kKeys);
+    if (p.D == 128 && f16) launch_wm<128, true>(pl.wm, p, maps, pl.ctas, device, stream);
+    else if (p.D == 128) launch_wm<128, false>(pl.wm, p, maps, pl.ctas, device, stream);
+    else if (f16) launch_wm<64, true>(pl.wm, p, maps, pl.ctas, device, stream);
+    else launch_wm<64, false>(pl.wm, p, maps, pl.ctas, device, stream);
+  }
   launch_combine(p, pl.ctas, f16, stream);
 }
 

@@ -265,6 +265,11 @@ struct KvMaps {
   int box;
 };
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys);
+// q [tokens, HQ, D] with token pitch ldq: boxes of tok x heads x 64
+CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int tok, int heads);
+// attention_paged_tc.cu
+void launch_tc(const krb_kv_cache &c, int layer, const Params &p, int ctas, int device,
+               cudaStream_t stream);
 size_t workspace_bytes(int ctas, int rows, int D);
 void carve_workspace(Params &p, int ctas, void *ws);
 

@@ -32,9 +32,9 @@ int sm_count(int device);
 CUtensorMap make_tmap_2d_bf16(const void *base, uint64_t rows, uint64_t cols, uint64_t ld,
                               uint32_t box_rows, uint32_t box_cols);
 // 4D map of a strided [n3, n2, n1, n0] array of 2-byte elements: dims innermost first,
-// strides of dims 1..3 in elements, box [box1, 64] of dims 1 and 0 (128-byte swizzle).
+// strides of dims 1..3 in elements, box [box2, box1, 64] of dims 2, 1, 0 (128-byte swizzle).
 CUtensorMap make_tmap_4d_2byte(const void *base, const uint64_t dims[4], const uint64_t strides[3],
-                               uint32_t box1);
+                               uint32_t box1, uint32_t box2 = 1);
 
 // ---- op launchers (all asynchronous on `stream`; shapes validated, throw on misuse)
 // C[M,N] = A[M,K] . B[N,K]^T (+bias[N]); lda/ldb/ldc in elements.

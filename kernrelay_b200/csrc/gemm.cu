@@ -93,7 +93,7 @@ CUtensorMap make_tmap_2d_bf16(const void *base, uint64_t rows, uint64_t cols, ui
 }
 
 CUtensorMap make_tmap_4d_2byte(const void *base, const uint64_t dims[4], const uint64_t strides[3],
-                               uint32_t box1) {
+                               uint32_t box1, uint32_t box2) {
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0) throw CudaError("tensor map base not 16B aligned");
   CUtensorMap m;
   const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
@@ -102,7 +102,7 @@ CUtensorMap make_tmap_4d_2byte(const void *base, const uint64_t dims[4], const u
     if (strides[i] % 8) throw CudaError("tensor map stride not a multiple of 16 bytes");
     st[i] = strides[i] * 2;
   }
-  const cuuint32_t box[4] = {64, box1, 1, 1};
+  const cuuint32_t box[4] = {64, box1, box2, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), d,
                                st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
