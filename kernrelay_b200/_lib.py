@@ -5,10 +5,10 @@ If the library is missing the import of the wrappers fails loudly.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import json
 import os
+from array import array
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -157,14 +157,22 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _empty(shape, dtype, device, stream):
-    """A tensor that this call's kernels on `stream` use: allocated on that stream, so that the
-    allocator does not hand its memory to another stream's work too early."""
-    import torch
+def _empty(shape, dtype, like, stream):
+    """A tensor on `like`'s device that this call's kernels on `stream` use: allocated on that
+    stream, so that the allocator does not hand its memory to another stream's work too early."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    import torch
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _raw_stream(stream, index):
+    """cudaStream_t of `stream`, or of the current stream of device `index`."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _stream(stream):
@@ -316,7 +324,7 @@ class KVCache:
             raise KrbError("KVCache: k and v on different devices")
         if k.stride(-1) != 1 or v.stride(-1) != 1:
             raise KrbError("KVCache: head_dim must be contiguous")
-        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        self.k, self.v, self.dtype, self.index = k, v, k.dtype, k.get_device()
         sizes = ((1,) + tuple(k.shape))[-5:]
         self.layers, self.pages, self.heads, self.page_size, self.head_dim = sizes
         strides = [((0,) + tuple(t.stride()))[-5:-1] for t in (k, v)]
@@ -329,7 +337,10 @@ class KVCache:
         """Bytes of attention_paged's workspace (krb_attention_paged_workspace)."""
         n = self._workspaces.get((HQ, max_q))
         if n is None:
-            with _on(self.device):
+            import torch
+            if self.index < 0:
+                raise KrbError("KVCache: the cache is not on a GPU")
+            with torch.cuda.device(self.index):
                 n = lib().krb_attention_paged_workspace(self.ref, HQ, max_q)
             if not n:
                 raise KrbError(lib().krb_last_error().decode(errors="replace"))
@@ -337,25 +348,33 @@ class KVCache:
         return n
 
 
-def _on(device):
-    """The device that the library's calls run on, where it is not the current one."""
-    import torch
-    if device.type != "cuda" or device.index in (None, torch.cuda.current_device()):
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _is(t, dtype, index, dim):
+    """A dim-d tensor of dtype on CUDA device `index` whose last axis is contiguous.  These
+    operators' smallest calls take a few microseconds, so their checks are kept as cheap."""
+    return (t.dtype is dtype and t.get_device() == index and t.dim() == dim
+            and (t.stride(-1) == 1 or t.size(-1) <= 1))
 
 
-def _want(what, name, t, dtype, device, dim, inner=True):
-    if t.dtype != dtype or t.device != device or t.dim() != dim or (
-            inner and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise KrbError(f"{what}: {name} must be a {dim}-d {dtype} tensor on {device} with its last "
-                       f"axis contiguous, got {t.dim()}-d {t.dtype} on {t.device}, strides "
-                       f"{tuple(t.stride())}")
+def _refuse(what, name, t, dtype, dim):
+    raise KrbError(f"{what}: {name} must be a {dim}-d {dtype} tensor on the cache's device with its "
+                   f"last axis contiguous, got {t.dim()}-d {t.dtype} on {t.device}, strides "
+                   f"{tuple(t.stride())}")
 
 
 def _pitch(t):
     """Row pitch of a 2-d tensor (rows that are never stepped over may have any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else width
+
+
+def _enter(cache):
+    """None where the cache's device is the current one, else the context to call again in."""
+    import torch
+    if cache.index < 0:
+        raise KrbError("KVCache: the cache is not on a GPU")
+    if torch.cuda.current_device() == cache.index:
+        return None
+    return torch.cuda.device(cache.index)
 
 
 def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, k_norm=None,
@@ -365,37 +384,44 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
     slots[n] = page * page_size + offset of the cache's `layer` (-1: not written).  positions and
     slots int64 [N]; cos / sin bf16 [max_pos, D]."""
     import torch
-    what = "qk_norm_rope_paged"
-    N, D, dev = qkv.shape[0], cache.head_dim, cache.device
-    _want(what, "qkv", qkv, cache.dtype, dev, 2)
-    if qkv.shape[1] != (HQ + 2 * cache.heads) * D:
+    what, dt, index, i64, bf = "qk_norm_rope_paged", cache.dtype, cache.index, torch.int64, torch.bfloat16
+    if not _is(qkv, dt, index, 2):
+        _refuse(what, "qkv", qkv, dt, 2)
+    if not _is(positions, i64, index, 1):
+        _refuse(what, "positions", positions, i64, 1)
+    if not _is(slots, i64, index, 1):
+        _refuse(what, "slots", slots, i64, 1)
+    if not _is(cos, bf, index, 2):
+        _refuse(what, "cos", cos, bf, 2)
+    if not _is(sin, bf, index, 2):
+        _refuse(what, "sin", sin, bf, 2)
+    D = cache.head_dim
+    N, width = qkv.shape
+    if width != (HQ + 2 * cache.heads) * D:
         raise KrbError(f"{what}: qkv rows must hold (HQ + 2*HKV) * head_dim values")
-    for name, t in (("positions", positions), ("slots", slots)):
-        _want(what, name, t, torch.int64, dev, 1)
-        if t.shape[0] != N:
-            raise KrbError(f"{what}: {name} must have one entry per row of qkv")
-    for name, t in (("cos", cos), ("sin", sin)):
-        _want(what, name, t, torch.bfloat16, dev, 2)
-        if t.shape != cos.shape or t.shape[1] != D or not t.is_contiguous():
-            raise KrbError(f"{what}: cos and sin must be contiguous [max_pos, head_dim]")
+    if len(positions) != N or len(slots) != N:
+        raise KrbError(f"{what}: positions and slots must have one entry per row of qkv")
+    max_pos = len(cos)
+    if (cos.shape != (max_pos, D) or sin.shape != (max_pos, D) or not cos.is_contiguous()
+            or not sin.is_contiguous()):
+        raise KrbError(f"{what}: cos and sin must be contiguous [max_pos, head_dim]")
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None:
-            _want(what, name, t, torch.bfloat16, dev, 1)
-            if t.shape[0] != D:
-                raise KrbError(f"{what}: {name} must have head_dim values")
-    if status is not None:
-        _want(what, "status", status, torch.int32, dev, 1)
-    with _on(dev):
-        if out is None:
-            out = _empty((N, HQ * D), cache.dtype, dev, stream)
-        else:
-            _want(what, "out", out, cache.dtype, dev, 2)
-            if out.shape != (N, HQ * D):
-                raise KrbError(f"{what}: out must be [N, HQ*head_dim]")
-        check(lib().krb_qk_norm_rope_paged(
-            cache.ref, layer, qkv.data_ptr(), _pitch(qkv), out.data_ptr(), _pitch(out),
-            positions.data_ptr(), slots.data_ptr(), N, HQ, cos.data_ptr(), sin.data_ptr(),
-            cos.shape[0], _addr(q_norm), _addr(k_norm), eps, _addr(status), _stream(stream)), what)
+        if t is not None and not (_is(t, bf, index, 1) and len(t) == D):
+            _refuse(what, f"{name} [head_dim]", t, bf, 1)
+    if status is not None and not _is(status, torch.int32, index, 1):
+        _refuse(what, "status", status, torch.int32, 1)
+    if out is not None and not (_is(out, dt, index, 2) and out.shape == (N, HQ * D)):
+        _refuse(what, "out [N, HQ*head_dim]", out, dt, 2)
+    if (on := _enter(cache)) is not None:
+        with on:
+            return qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm, k_norm,
+                                      eps, layer, out, status, stream)
+    if out is None:
+        out = _empty((N, HQ * D), dt, qkv, stream)
+    check(lib().krb_qk_norm_rope_paged(
+        cache.ref, layer, qkv.data_ptr(), _pitch(qkv), out.data_ptr(), _pitch(out),
+        positions.data_ptr(), slots.data_ptr(), N, HQ, cos.data_ptr(), sin.data_ptr(), max_pos,
+        _addr(q_norm), _addr(k_norm), eps, _addr(status), _raw_stream(stream, index)), what)
     return out
 
 
@@ -409,44 +435,50 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
     than any T_b.  workspace: a uint8 tensor of cache.attention_workspace(HQ, max_q) bytes that no
     other call uses until this one is done (default: allocated per call)."""
     import torch
-    what = "attention_paged"
-    dev, i32 = cache.device, torch.int32
-    _want(what, "q", q, cache.dtype, dev, 2)
+    what, dt, index, i32 = "attention_paged", cache.dtype, cache.index, torch.int32
+    if not _is(q, dt, index, 2):
+        _refuse(what, "q", q, dt, 2)
+    if not _is(page_table, i32, index, 2):
+        _refuse(what, "page_table", page_table, i32, 2)
+    if not _is(kv_lens, i32, index, 1):
+        _refuse(what, "kv_lens", kv_lens, i32, 1)
+    if not _is(q_starts, i32, index, 1):
+        _refuse(what, "q_starts", q_starts, i32, 1)
     N, width = q.shape
     HQ = width // cache.head_dim
     if HQ * cache.head_dim != width:
         raise KrbError(f"{what}: q rows must hold HQ * head_dim values")
-    _want(what, "page_table", page_table, i32, dev, 2)
-    _want(what, "kv_lens", kv_lens, i32, dev, 1)
-    _want(what, "q_starts", q_starts, i32, dev, 1)
-    B = kv_lens.shape[0]
-    if page_table.shape[0] != B or q_starts.shape[0] != B + 1:
+    B, max_pages = page_table.shape
+    if len(kv_lens) != B or len(q_starts) != B + 1:
         raise KrbError(f"{what}: page_table, kv_lens and q_starts must be of the same batch")
-    words = 0
+    words = ldm = 0
     if mask is not None:
-        _want(what, "mask", mask, i32, dev, 2)
-        if mask.shape[0] != N:
+        if not _is(mask, i32, index, 2):
+            _refuse(what, "mask", mask, i32, 2)
+        rows, words = mask.shape
+        if rows != N:
             raise KrbError(f"{what}: mask must have one row per row of q")
-        words = mask.shape[1]
-    if status is not None:
-        _want(what, "status", status, i32, dev, 1)
+        ldm = _pitch(mask)
+    if status is not None and not _is(status, i32, index, 1):
+        _refuse(what, "status", status, i32, 1)
+    if out is not None and not (_is(out, dt, index, 2) and out.shape == q.shape):
+        _refuse(what, "out [N, HQ*head_dim]", out, dt, 2)
+    if workspace is not None and not _is(workspace, torch.uint8, index, 1):
+        _refuse(what, "workspace", workspace, torch.uint8, 1)
+    if (on := _enter(cache)) is not None:
+        with on:
+            return attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask,
+                                   layer, out, workspace, status, stream)
     need = cache.attention_workspace(HQ, max_q)
-    with _on(dev):
-        if out is None:
-            out = _empty((N, width), cache.dtype, dev, stream)
-        else:
-            _want(what, "out", out, cache.dtype, dev, 2)
-            if out.shape != q.shape:
-                raise KrbError(f"{what}: out must have q's shape")
-        if workspace is None:
-            workspace = _empty((need,), torch.uint8, dev, stream)
-        else:
-            _want(what, "workspace", workspace, torch.uint8, dev, 1)
-        check(lib().krb_attention_paged(
-            cache.ref, layer, q.data_ptr(), _pitch(q), out.data_ptr(), _pitch(out), N, HQ,
-            page_table.data_ptr(), _pitch(page_table), page_table.shape[1], kv_lens.data_ptr(),
-            q_starts.data_ptr(), B, max_q, _addr(mask), _pitch(mask) if words else 0, words, scale,
-            workspace.data_ptr(), workspace.numel(), _addr(status), _stream(stream)), what)
+    if out is None:
+        out = _empty((N, width), dt, q, stream)
+    if workspace is None:
+        workspace = _empty((need,), torch.uint8, q, stream)
+    check(lib().krb_attention_paged(
+        cache.ref, layer, q.data_ptr(), _pitch(q), out.data_ptr(), _pitch(out), N, HQ,
+        page_table.data_ptr(), _pitch(page_table), max_pages, kv_lens.data_ptr(),
+        q_starts.data_ptr(), B, max_q, _addr(mask), ldm, words, scale, workspace.data_ptr(),
+        len(workspace), _addr(status), _raw_stream(stream, index)), what)
     return out
 
 
@@ -454,17 +486,20 @@ def kv_copy_pages(cache, src, dst, stream=None):
     """Copy page src[i] to page dst[i], K and V of all layers (a fork's page of its own, or pages
     moved together).  src, dst: host sequences of page numbers; no page is written twice, or both
     read and written."""
-    n = len(src)
+    what, n = "kv_copy_pages", len(src)
     if len(dst) != n:
-        raise KrbError("kv_copy_pages: src and dst differ in length")
+        raise KrbError(f"{what}: src and dst differ in length")
+    if getattr(src, "is_cuda", False) or getattr(dst, "is_cuda", False):
+        raise KrbError(f"{what}: src and dst must be host integers, not tensors on a GPU")
     try:
-        pages = (c_int * (2 * n))(*src, *dst)
-    except TypeError as e:
-        raise KrbError(f"kv_copy_pages: src and dst must be host integers ({e})") from None
-    at = ctypes.addressof(pages)
-    with _on(cache.device):
-        check(lib().krb_kv_copy_pages(cache.ref, at, at + 4 * n, n, _stream(stream)),
-              "kv_copy_pages")
+        src, dst = (array("i", x.tolist() if hasattr(x, "tolist") else x) for x in (src, dst))
+    except (TypeError, OverflowError) as e:
+        raise KrbError(f"{what}: src and dst must be host integers ({e})") from None
+    if (on := _enter(cache)) is not None:
+        with on:
+            return kv_copy_pages(cache, src, dst, stream)
+    check(lib().krb_kv_copy_pages(cache.ref, src.buffer_info()[0], dst.buffer_info()[0], n,
+                                  _raw_stream(stream, cache.index)), what)
 
 
 def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=None):
@@ -472,22 +507,28 @@ def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=No
     move to position bases[b] + i for i < counts[b], all layers.  accepted int32 [B, A], ascending
     strictly from >= 0 per sequence; bases, counts int32 [B]; page_table as in attention_paged."""
     import torch
-    what = "kv_commit"
-    dev, i32 = cache.device, torch.int32
-    _want(what, "page_table", page_table, i32, dev, 2)
-    _want(what, "accepted", accepted, i32, dev, 2)
-    _want(what, "bases", bases, i32, dev, 1)
-    _want(what, "counts", counts, i32, dev, 1)
+    what, index, i32 = "kv_commit", cache.index, torch.int32
+    if not _is(page_table, i32, index, 2):
+        _refuse(what, "page_table", page_table, i32, 2)
+    if not _is(accepted, i32, index, 2):
+        _refuse(what, "accepted", accepted, i32, 2)
+    if not _is(bases, i32, index, 1):
+        _refuse(what, "bases", bases, i32, 1)
+    if not _is(counts, i32, index, 1):
+        _refuse(what, "counts", counts, i32, 1)
     B, A = accepted.shape
-    if page_table.shape[0] != B or bases.shape[0] != B or counts.shape[0] != B:
+    rows, max_pages = page_table.shape
+    if rows != B or len(bases) != B or len(counts) != B:
         raise KrbError(f"{what}: page_table, bases, accepted and counts must be of the same batch")
-    if status is not None:
-        _want(what, "status", status, i32, dev, 1)
-    with _on(dev):
-        check(lib().krb_kv_commit(
-            cache.ref, page_table.data_ptr(), _pitch(page_table), page_table.shape[1],
-            bases.data_ptr(), accepted.data_ptr(), _pitch(accepted), A, counts.data_ptr(), B,
-            _addr(status), _stream(stream)), what)
+    if status is not None and not _is(status, i32, index, 1):
+        _refuse(what, "status", status, i32, 1)
+    if (on := _enter(cache)) is not None:
+        with on:
+            return kv_commit(cache, page_table, bases, accepted, counts, status, stream)
+    check(lib().krb_kv_commit(
+        cache.ref, page_table.data_ptr(), _pitch(page_table), max_pages, bases.data_ptr(),
+        accepted.data_ptr(), _pitch(accepted), A, counts.data_ptr(), B, _addr(status),
+        _raw_stream(stream, index)), what)
 
 
 def relay_down_single(act, w_down, resid, gamma, tiles, eps, bn=0, status=None, stream=None):
