@@ -30,7 +30,7 @@ struct Cfg {
   static constexpr int kMerge = kMergeLane * 32 * 4;    // bytes per sending warp
   static constexpr int kBars = 2 * kStages * 8;
   static constexpr int kSmem =
-      2 * kStages * kTile + 2 * kMerge + kBars + int(sizeof(WalkStart)) + 16 + 1024;
+      2 * kStages * kTile + 2 * kMerge + kBars + int(sizeof(Walk)) + 16 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   float *merge = reinterpret_cast<float *>(smem + 2 * C::kStages * C::kTile);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + 2 * C::kStages * C::kTile + 2 * C::kMerge);
   uint64_t *empty = full + C::kStages;
-  WalkStart *start = reinterpret_cast<WalkStart *>(empty + C::kStages);
+  Walk *start = reinterpret_cast<Walk *>(empty + C::kStages);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
@@ -103,11 +103,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     fence_mbar_init();
   }
   if (warp == 4) {
-    const WalkStart s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
+    const Walk s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
     if (lane == 0) *start = s;
   }
   __syncthreads();
-  Walk w = begin_walk<kKeys>(p, *start);
+  Walk w = *start;
 
   if (warp == 4) {
     // ---------------- producer: one TMA box per lane (page x half x K or V)
@@ -122,11 +122,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     while (w.pos < w.end && ok) {
       const int e = piece_end(w);
       const int end = kv_end(p, w.T, w.ctx, w.i);
+      auto boxes = [&](int blk) { return (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift; };
+      auto page_at = [&](int blk) {
+        return blk < e && bx < boxes(blk) ? page_of(p, w.b, blk * kKeys + (bx << box_shift)) : 0;
+      };
+      int next_page = page_at(w.blk);
       for (int blk = w.blk; blk < e; ++blk, ++n) {
         const int s = n % C::kStages;
         const int key = blk * kKeys + (bx << box_shift);
-        const int nbox = (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift;
-        const int page = bx < nbox ? page_of(p, w.b, key) : 0;
+        const int nbox = boxes(blk);
+        const int page = next_page;
+        next_page = page_at(blk + 1);  // in flight while this block waits for its stage
         ok = mbar_wait(&empty[s], ((n / C::kStages) & 1) ^ 1, kMbarLimitNs);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -210,16 +216,22 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int x = 0; x < 4; ++x) sc[t][x] = 0.f;
+        // fragments are fetched a step ahead: two warps per scheduler do not hide ldmatrix
         const int krow = wn * kWarpKeys + (lane >> 4) * 8 + (lane & 7);
+        uint32_t kb[2][NT / 2][4];
+        auto load_k = [&](int ks) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
+          for (int t = 0; t < NT; t += 2)
+            ldsm4(kt + tile_off<D>(krow + t * 8, 2 * ks + ((lane >> 3) & 1)), kb[ks & 1][t / 2]);
+        };
+        load_k(0);
 #pragma unroll
-          for (int t = 0; t < NT; t += 2) {
-            uint32_t b[4];
-            ldsm4(kt + tile_off<D>(krow + t * 8, 2 * ks + ((lane >> 3) & 1)), b);
-            mma16816<F16>(sc[t], qf[ks], b[0], b[1]);
-            mma16816<F16>(sc[t + 1], qf[ks], b[2], b[3]);
-          }
+        for (int ks = 0; ks < D / 16; ++ks) {
+          if (ks + 1 < D / 16) load_k(ks + 1);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            mma16816<F16>(sc[t], qf[ks], kb[ks & 1][t / 2][(t & 1) * 2], kb[ks & 1][t / 2][(t & 1) * 2 + 1]);
+        }
         // the first row's token decides whether anything of these keys is hidden
         if (k0 + kWarpKeys > w.ctx + (p.mask ? 0 : tok0 + 1)) {
 #pragma unroll
@@ -237,6 +249,16 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
+        constexpr int kVSteps = D / 32;  // steps of 16 keys x 32 columns
+        const int vrow = wn * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
+        uint32_t vb[2][2][4];
+        auto load_v = [&](int i) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+            ldsm4_t(vt + tile_off<D>(vrow + i / kVSteps * 16, (i % kVSteps) * 4 + d * 2 + (lane >> 4)),
+                    vb[i & 1][d]);
+        };
+        load_v(0);
         float mx[2] = {m[0], m[1]};
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -280,16 +302,14 @@ __global__ void __launch_bounds__(kThreads, 2)
             pf[t / 2][(t & 1) * 2 + x] = pack2<F16>(p0, p1);
           }
         }
-        const int vrow = wn * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
-        for (int ks = 0; ks < NT / 2; ++ks)
+        for (int i = 0; i < NT / 2 * kVSteps; ++i) {
+          if (i + 1 < NT / 2 * kVSteps) load_v(i + 1);
+          const int ks = i / kVSteps, d0 = i % kVSteps * 4;
 #pragma unroll
-          for (int d = 0; d < DT; d += 2) {
-            uint32_t b[4];
-            ldsm4_t(vt + tile_off<D>(vrow + ks * 16, d + (lane >> 4)), b);
-            mma16816<F16>(o[d], pf[ks], b[0], b[1]);
-            mma16816<F16>(o[d + 1], pf[ks], b[2], b[3]);
-          }
+          for (int d = 0; d < 4; ++d)
+            mma16816<F16>(o[d0 + d], pf[ks], vb[i & 1][d / 2][(d & 1) * 2], vb[i & 1][d / 2][(d & 1) * 2 + 1]);
+        }
       }
       if (wrote) fence_proxy_async_shared();
       __syncwarp();
@@ -396,45 +416,74 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ------------------------------------------------------------------ joining split units
-// CTA (c, y) joins rows y * 4 .. of the unit that CTA c of the attention kernel began and later
-// ones went on with: a warp per row, O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-template <int D, bool F16>
+// CTA (c, y) joins rows y * 4 / KW .. of the unit that CTA c of the attention kernel began and later
+// ones went on with: KW warps per row, each every KW-th piece, then their sums in order;
+// O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.  A long sequence over few units is cut into
+// dozens of pieces (KW = 4: few rows), a wide draft into two or three (KW = 1).
+template <int D, int KW, bool F16>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   constexpr int V = D / 32;  // columns of a lane
+  constexpr int kUnroll = 4;
+  __shared__ float part[4][32][V + 1];
   pdl_wait();
   const int c = blockIdx.x;
   const int4 d = p.desc[c];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.y * 4 + warp;
-  if (d.w < 2 || r >= d.y * p.group) return;
+  const int r = (blockIdx.y * 4 + warp) / KW, kw = warp % KW;
+  if (d.w < 2 || (blockIdx.y * 4) / KW >= d.y * p.group) return;
+  const bool row_ok = r < d.y * p.group;
   const int tok = r / p.group, g = r - tok * p.group;
-  const int sr = slot_row(p, tok, g);
+  const int sr = row_ok ? slot_row(p, tok, g) : 0;
+  const int pieces = row_ok ? d.w : 0;
   float mx = -INFINITY;
-  for (int k = lane; k < d.w; k += 32) mx = fmaxf(mx, slot_ml(p, c + k, k == 0)[sr]);
+  for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, slot_ml(p, c + k, k == 0)[sr]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float off = mx == -INFINITY ? 0.f : mx;
   float total = 0.f, acc[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) acc[x] = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < d.w; ++k) {
-    const float *ml = slot_ml(p, c + k, k == 0);
-    const float f = exp2_mufu(ml[sr] - off);
-    total += f * ml[p.rows + sr];
-    const float *o = slot_o(p, c + k, k == 0) + static_cast<long>(sr) * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 v = *reinterpret_cast<const float4 *>(o);
-      acc[0] += f * v.x;
-      acc[1] += f * v.y;
-      acc[2] += f * v.z;
-      acc[3] += f * v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2 *>(o);
-      acc[0] += f * v.x;
-      acc[1] += f * v.y;
+  for (int k0 = kw; k0 < pieces; k0 += KW * kUnroll) {
+    float f[kUnroll], l[kUnroll], v[kUnroll][V];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int k = k0 + u * KW;
+      if (k >= pieces) continue;
+      const float *ml = slot_ml(p, c + k, k == 0);
+      f[u] = ml[sr];
+      l[u] = ml[p.rows + sr];
+      const float *o = slot_o(p, c + k, k == 0) + static_cast<long>(sr) * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 t = *reinterpret_cast<const float4 *>(o);
+        v[u][0] = t.x, v[u][1] = t.y, v[u][2] = t.z, v[u][3] = t.w;
+      } else {
+        const float2 t = *reinterpret_cast<const float2 *>(o);
+        v[u][0] = t.x, v[u][1] = t.y;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (k0 + u * KW >= pieces) continue;
+      const float w = exp2_mufu(f[u] - off);
+      total += w * l[u];
+#pragma unroll
+      for (int x = 0; x < V; ++x) acc[x] += w * v[u][x];
     }
   }
+  if constexpr (KW > 1) {
+#pragma unroll
+    for (int x = 0; x < V; ++x) part[warp][lane][x] = acc[x];
+    part[warp][lane][V] = total;
+    __syncthreads();
+    if (kw != 0) return;
+#pragma unroll
+    for (int k = 1; k < KW; ++k) {
+#pragma unroll
+      for (int x = 0; x < V; ++x) acc[x] += part[warp + k][lane][x];
+      total += part[warp + k][lane][V];
+    }
+  }
+  if (!row_ok) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   uint16_t *out = p.out + (d.x + tok) * p.ldo + static_cast<long>(d.z * p.group + g) * D + lane * V;
   if constexpr (V == 4)
@@ -445,9 +494,11 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ host side
-void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
+template <int KW>
+static void combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
+  const int rows = std::min(p.tpt, p.max_q) * p.group;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, (p.tpt * p.group + 3) / 4);
+  cfg.gridDim = dim3(ctas, (rows * KW + 3) / 4);
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -455,9 +506,14 @@ void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, true> : combine_kernel<128, false>)
-                          : (f16 ? combine_kernel<64, true> : combine_kernel<64, false>);
+  auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, KW, true> : combine_kernel<128, KW, false>)
+                          : (f16 ? combine_kernel<64, KW, true> : combine_kernel<64, KW, false>);
   KRB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+static void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
+  if (p.rows <= 16) combine<4>(p, ctas, f16, stream);
+  else combine<1>(p, ctas, f16, stream);
 }
 
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys) {

@@ -73,103 +73,90 @@ __device__ __forceinline__ long blocks_per_head(const Params &p, int T, int ctx)
 
 // A CTA's place on the line, kept by every role of the CTA alike.
 struct Walk {
-  int b, h, i;       // current unit
-  int q0, T, ctx;    // its sequence
-  int blk, nblk;     // next block of the unit to take, its blocks
-  long pos, end, per;  // line position of `blk`, this CTA's end, blocks per CTA
+  int b, h, i;        // current unit
+  int q0, T, ctx;     // its sequence
+  int blk, nblk;      // next block of the unit to take, its blocks
+  int pos, end, per;  // line position of `blk`, this CTA's end, blocks per CTA
 };
 
-struct WalkStart {
-  int b, h, i, blk;
-  long pos, end, per;
-};
+// One warp finds the CTA's start (all lanes return it).  Everything waits for this, so the sums
+// are 32 bits wide: a sequence of more than kMostBlocks blocks, or a batch of 2^31, is refused.
+constexpr long kMostBlocks = 1L << 26;
 
-// One warp finds the CTA's start (all lanes return it).
 template <int kKeys>
-__device__ __forceinline__ WalkStart find_start(const Params &p, int cta, int ctas) {
+__device__ __forceinline__ Walk find_start(const Params &p, int cta, int ctas) {
   const int lane = threadIdx.x & 31;
+  Seq s{0, 0, 0};
+  uint32_t n = 0, per_head = 0;  // of sequence b0 + lane
+  bool bad = false;
+  auto load = [&](int b0, bool report) {
+    s = Seq{0, 0, 0};
+    n = per_head = 0;
+    if (b0 + lane < p.B) {
+      s = load_seq(p, b0 + lane, report);
+      if (s.T) {
+        const long k = blocks_per_head<kKeys>(p, s.T, s.ctx);
+        bad |= k * p.HKV > kMostBlocks;
+        per_head = static_cast<uint32_t>(k);
+        n = bad ? 0 : per_head * p.HKV;
+      }
+    }
+  };
   long total = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    long n = 0;
-    if (b0 + lane < p.B) {
-      const Seq s = load_seq(p, b0 + lane, cta == 0);
-      if (s.T) n = blocks_per_head<kKeys>(p, s.T, s.ctx) * p.HKV;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
+    load(b0, cta == 0);
+    total += __reduce_add_sync(0xffffffffu, n);
   }
-  WalkStart w{0, 0, 0, 0, 0, 0, 1};
+  Walk w{};
+  w.per = 1;
+  if (__any_sync(0xffffffffu, bad) || total > 0x7fffffffL) {
+    if (cta == 0 && lane == 0) report_status(p.status, kStatusBadArgs);
+    return w;
+  }
   if (total == 0) return w;
-  w.per = (total + ctas - 1) / ctas;
-  w.pos = min(total, w.per * cta);
-  w.end = min(total, w.pos + w.per);
+  const uint32_t tot = static_cast<uint32_t>(total), per = (tot + ctas - 1) / ctas;
+  const uint32_t pos = min(static_cast<unsigned long long>(per) * cta, static_cast<unsigned long long>(tot));
+  w.per = per;
+  w.pos = pos;
+  w.end = min(tot, pos + per);
   if (w.pos >= w.end) return w;
-  long before = 0;
+  uint32_t before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    long n = 0, per_head = 0;
-    Seq s{0, 0, 0};
-    if (b0 + lane < p.B) {
-      s = load_seq(p, b0 + lane, false);
-      if (s.T) per_head = blocks_per_head<kKeys>(p, s.T, s.ctx);
-      n = per_head * p.HKV;
-    }
-    long incl = n;
+    if (p.B > 32) load(b0, false);
+    uint32_t incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long v = __shfl_up_sync(0xffffffffu, incl, o);
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w.pos);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > pos);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      const long excl = __shfl_sync(0xffffffffu, incl - n, l);
-      per_head = __shfl_sync(0xffffffffu, per_head, l);
-      const int T = __shfl_sync(0xffffffffu, s.T, l), ctx = __shfl_sync(0xffffffffu, s.ctx, l);
-      long rem = w.pos - before - excl;
+      uint32_t rem = pos - before - __shfl_sync(0xffffffffu, incl - n, l);
+      const uint32_t ph = __shfl_sync(0xffffffffu, per_head, l);
+      w.q0 = __shfl_sync(0xffffffffu, s.q0, l);
+      w.T = __shfl_sync(0xffffffffu, s.T, l);
+      w.ctx = __shfl_sync(0xffffffffu, s.ctx, l);
       w.b = b0 + l;
-      w.h = static_cast<int>(rem / per_head);
-      rem -= w.h * per_head;
-      for (;;) {
-        const int nb = (kv_end(p, T, ctx, w.i) + kKeys - 1) / kKeys;
-        if (rem < nb) break;
-        rem -= nb;
-        ++w.i;
+      w.h = rem / ph;
+      rem -= w.h * ph;
+      for (;; ++w.i) {
+        w.nblk = (kv_end(p, w.T, w.ctx, w.i) + kKeys - 1) / kKeys;
+        if (rem < static_cast<uint32_t>(w.nblk)) break;
+        rem -= w.nblk;
       }
-      w.blk = static_cast<int>(rem);
+      w.blk = rem;
       return w;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  w.pos = w.end = 0;
-  return w;
-}
-
-template <int kKeys>
-__device__ __forceinline__ Walk begin_walk(const Params &p, const WalkStart &s) {
-  Walk w;
-  w.b = s.b;
-  w.h = s.h;
-  w.i = s.i;
-  w.blk = s.blk;
-  w.pos = s.pos;
-  w.end = s.end;
-  w.per = s.per;
-  w.q0 = w.T = w.ctx = w.nblk = 0;
-  if (w.pos < w.end) {
-    const Seq q = load_seq(p, w.b, false);
-    w.q0 = q.q0;
-    w.T = q.T;
-    w.ctx = q.ctx;
-    w.nblk = (kv_end(p, w.T, w.ctx, w.i) + kKeys - 1) / kKeys;
-  }
+  w.pos = w.end = 0;  // not reached: the line ends behind its last sequence
   return w;
 }
 
 // this CTA's blocks of the current unit: [w.blk, piece_end(w))
 __device__ __forceinline__ int piece_end(const Walk &w) {
-  const long left = w.end - w.pos;
-  return w.nblk - w.blk <= left ? w.nblk : w.blk + static_cast<int>(left);
+  return min(w.nblk, w.blk + (w.end - w.pos));
 }
 
 // the unit after the piece that ends at block `e` (only when the CTA has blocks left)
@@ -189,7 +176,7 @@ __device__ __forceinline__ void next_unit(const Params &p, Walk &w, int e) {
         w.T = q.T;
         w.ctx = q.ctx;
       }
-      if (!w.T) {  // not reached: the line ends with the last sequence
+      if (!w.T) {  // not reached: the line ends behind its last sequence
         w.pos = w.end;
         return;
       }
@@ -224,11 +211,10 @@ __device__ __forceinline__ int page_of(const Params &p, int b, int key) {
 // What the combine kernel needs of a unit that CTA c starts and later CTAs go on with.
 __device__ __forceinline__ int4 split_desc(const Params &p, const Walk &w) {
   // unit's end on the line; its last CTA holds position end - 1
-  const long end = w.pos - w.blk + w.nblk;
-  const int last = static_cast<int>((end - 1) / w.per);
-  const int first = static_cast<int>(w.pos / w.per);
+  const uint32_t end = w.pos - w.blk + w.nblk, per = w.per;
   const int tok0 = w.i * p.tpt;
-  return make_int4(w.q0 + tok0, min(p.tpt, w.T - tok0), w.h, last - first + 1);
+  return make_int4(w.q0 + tok0, min(p.tpt, w.T - tok0), w.h,
+                   static_cast<int>((end - 1) / per - w.pos / per) + 1);
 }
 
 __device__ __forceinline__ float *slot_ml(const Params &p, int cta, int slot) {
@@ -256,10 +242,7 @@ __device__ __forceinline__ float exp2_mufu(float x) {
   return y;
 }
 
-// Host side.  Joins the split units of a launch of `ctas` CTAs (programmatic dependent launch:
-// its CTAs are set up while the attention kernel drains).
-void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream);
-// the tensor maps of one layer's K and V, boxes of min(page_size, keys) slots
+// Host side: the tensor maps of one layer's K and V, boxes of min(page_size, keys) slots
 struct KvMaps {
   CUtensorMap k, v;
   int box;

@@ -35,7 +35,7 @@ struct Cfg {
   static constexpr int kThreads = 64 + 128 * NT;
   static constexpr int kBars = 2 * kSlots + 2 + 3 * NT;
   static constexpr int kSmem =
-      (NT + kSlots) * kTile + kBars * 8 + int(sizeof(WalkStart)) + 32 + 1024;
+      (NT + kSlots) * kTile + kBars * 8 + int(sizeof(Walk)) + 32 + 1024;
 };
 
 // D[tmem] (+)= A[tmem] * B[smem], A 16-bit pairs K-major
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
   uint64_t *s_full = q_empty + 1;
   uint64_t *p_ready = s_full + NT;
   uint64_t *o_done = p_ready + NT;
-  WalkStart *start = reinterpret_cast<WalkStart *>(o_done + NT);
+  Walk *start = reinterpret_cast<Walk *>(o_done + NT);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(start + 1);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
     }
-    const WalkStart s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
+    const Walk s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
     if (lane == 0) *start = s;
   } else if (warp == 1) {
     __syncwarp();
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Walk w = begin_walk<kKeys>(p, *start);
+  Walk w = *start;
 
   if (warp == 0) {
     // ---------------- TMA producer: a box (page x 64 columns) per lane
