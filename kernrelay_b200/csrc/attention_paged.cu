@@ -30,7 +30,7 @@ struct Cfg {
   static constexpr int kMerge = kMergeLane * 32 * 4;    // bytes per sending warp
   static constexpr int kBars = 2 * kStages * 8;
   static constexpr int kSmem =
-      2 * kStages * kTile + 2 * kMerge + kBars + int(sizeof(Walk)) + 16 + 1024;
+      2 * kStages * kTile + 2 * kMerge + kBars + 5 * int(sizeof(Walk)) + 16 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -102,14 +102,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     fence_mbar_init();
   }
+  if (warp < 4) prefetch_page_table(p, threadIdx.x, kConsumers);
   if (warp == 4) {
     const Walk s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
     if (lane == 0) *start = s;
   }
   __syncthreads();
-  Walk w = *start;
 
   if (warp == 4) {
+    Walk w = *start;
     // ---------------- producer: one TMA box per lane (page x half x K or V)
     constexpr int kKinds = D / 64 * 2;
     const int box = 1 << box_shift;
@@ -117,22 +118,18 @@ __global__ void __launch_bounds__(kThreads, 2)
     const bool is_v = kind >= D / 64;
     const int half = kind % (D / 64);
     const CUtensorMap *map = is_v ? &tm_v : &tm_k;
+    PageFeed feed;
     int n = 0;  // blocks issued
     bool ok = true;
     while (w.pos < w.end && ok) {
       const int e = piece_end(w);
       const int end = kv_end(p, w.T, w.ctx, w.i);
-      auto boxes = [&](int blk) { return (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift; };
-      auto page_at = [&](int blk) {
-        return blk < e && bx < boxes(blk) ? page_of(p, w.b, blk * kKeys + (bx << box_shift)) : 0;
-      };
-      int next_page = page_at(w.blk);
+      feed.begin(p, w.b, w.blk * kKeys, min(end, e * kKeys));
       for (int blk = w.blk; blk < e; ++blk, ++n) {
         const int s = n % C::kStages;
         const int key = blk * kKeys + (bx << box_shift);
-        const int nbox = boxes(blk);
-        const int page = next_page;
-        next_page = page_at(blk + 1);  // in flight while this block waits for its stage
+        const int nbox = (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift;
+        const int page = feed.page(p, blk * kKeys, key);
         ok = mbar_wait(&empty[s], ((n / C::kStages) & 1) ^ 1, kMbarLimitNs);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -158,28 +155,47 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int wm = warp % WM, wn = warp / WM;
   const int g = lane >> 2, c2 = (lane & 3) * 2;
   const uint32_t base = smem_u32(smem);
+  // the walk lies in shared memory, a copy per warp: the block loop wants the registers
+  volatile Walk *vw = start + 1 + warp;
+  auto load_walk = [&] {
+    Walk w;
+    w.b = vw->b, w.h = vw->h, w.i = vw->i, w.q0 = vw->q0, w.T = vw->T, w.ctx = vw->ctx;
+    w.blk = vw->blk, w.nblk = vw->nblk, w.pos = vw->pos, w.end = vw->end, w.per = vw->per;
+    return w;
+  };
+  auto store_walk = [&](const Walk &w) {
+    __syncwarp();
+    if (lane == 0) {
+      vw->b = w.b, vw->h = w.h, vw->i = w.i, vw->q0 = w.q0, vw->T = w.T, vw->ctx = w.ctx;
+      vw->blk = w.blk, vw->nblk = w.nblk, vw->pos = w.pos, vw->end = w.end, vw->per = w.per;
+    }
+    __syncwarp();
+  };
+  store_walk(*start);
   int n = 0;
   bool ok = true;
-  while (w.pos < w.end) {
-    const int e = piece_end(w);
-    const int end = kv_end(p, w.T, w.ctx, w.i);
-    const int tok0 = w.i * p.tpt;
-    const int nrows = min(p.tpt, w.T - tok0) * p.group;
-    // rows g and g + 8 of this warp's tile: token and head
-    int tok[2], hd[2];
-    bool row_ok[2];
+  while (vw->pos < vw->end) {
+    int e, end, first_hidden;  // piece's end; unit's last key + 1; first key that a row may not see
     uint32_t qf[D / 16][4];
+    {
+      const Walk w = load_walk();
+      e = piece_end(w);
+      end = kv_end(p, w.T, w.ctx, w.i);
+      const int tok0 = w.i * p.tpt;
+      first_hidden = w.ctx + (p.mask ? 0 : tok0 + 1);
+      const int nrows = min(p.tpt, w.T - tok0) * p.group;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = wm * 16 + g + 8 * x;
-      row_ok[x] = r < nrows;
-      tok[x] = tok0 + r / p.group;
-      hd[x] = w.h * p.group + r % p.group;
-      const uint16_t *q = p.q + (w.q0 + tok[x]) * p.ldq + static_cast<long>(hd[x]) * D + c2;
+      for (int x = 0; x < 2; ++x) {
+        // rows g and g + 8 of this warp's tile
+        const int r = wm * 16 + g + 8 * x;
+        const bool there = r < nrows;
+        const uint16_t *q = p.q + (w.q0 + tok0 + r / p.group) * p.ldq +
+                            static_cast<long>(w.h * p.group + r % p.group) * D + c2;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        qf[ks][x] = row_ok[x] ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16)) : 0u;
-        qf[ks][2 + x] = row_ok[x] ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16 + 8)) : 0u;
+        for (int ks = 0; ks < D / 16; ++ks) {
+          qf[ks][x] = there ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16)) : 0u;
+          qf[ks][2 + x] = there ? __ldg(reinterpret_cast<const uint32_t *>(q + ks * 16 + 8)) : 0u;
+        }
       }
     }
     float o[DT][4];
@@ -189,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    for (int blk = w.blk; blk < e; ++blk, ++n) {
+    for (int blk = vw->blk; blk < e; ++blk, ++n) {
       const int s = n % C::kStages;
       if (ok) ok = mbar_wait(&full[s], (n / C::kStages) & 1, kMbarLimitNs);
       if (!__all_sync(0xffffffffu, ok)) {  // leave the waits, keep the CTA's barriers in step
@@ -232,20 +248,21 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int t = 0; t < NT; ++t)
             mma16816<F16>(sc[t], qf[ks], kb[ks & 1][t / 2][(t & 1) * 2], kb[ks & 1][t / 2][(t & 1) * 2 + 1]);
         }
-        // the first row's token decides whether anything of these keys is hidden
-        if (k0 + kWarpKeys > w.ctx + (p.mask ? 0 : tok0 + 1)) {
+        if (k0 + kWarpKeys > first_hidden) {
+          const int T = vw->T, ctx = vw->ctx, tok0 = vw->i * p.tpt;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
+            const int t = tok0 + (wm * 16 + g + 8 * x) / p.group;
             const uint32_t *row_mask =
-                p.mask ? p.mask + (w.q0 + (row_ok[x] ? tok[x] : tok0)) * p.ldm : nullptr;
+                p.mask ? p.mask + (vw->q0 + (t < T ? t : tok0)) * p.ldm : nullptr;
 #pragma unroll
             for (int k = 0; k < kWarpKeys; k += 32) {
-              const uint32_t see = visible32(p, row_mask, w.T, tok[x], k0 + k - w.ctx);
+              const uint32_t see = visible32(p, row_mask, T, t, k0 + k - ctx);
 #pragma unroll
-              for (int t = k / 8; t < NT && t < k / 8 + 4; ++t)
+              for (int t8 = k / 8; t8 < NT && t8 < k / 8 + 4; ++t8)
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
-                  if (!((see >> (t * 8 - k + c2 + y)) & 1)) sc[t][2 * x + y] = -INFINITY;
+                  if (!((see >> (t8 * 8 - k + c2 + y)) & 1)) sc[t8][2 * x + y] = -INFINITY;
             }
           }
         }
@@ -373,27 +390,27 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
 
+    Walk w = load_walk();
     if (wn == 0 && ok) {
       const bool whole = w.blk == 0 && e == w.nblk;
-      if (whole) {
+      const int tok0 = w.i * p.tpt;
+      const int nrows = min(p.tpt, w.T - tok0) * p.group;
+      const int slot = w.blk == 0;
+      float *ml = slot_ml(p, blockIdx.x, slot);
+      float *po = slot_o(p, blockIdx.x, slot);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (!row_ok[x]) continue;
+      for (int x = 0; x < 2; ++x) {
+        const int r = wm * 16 + g + 8 * x;
+        if (r >= nrows) continue;
+        if (whole) {
           const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
-          uint16_t *out = p.out + (w.q0 + tok[x]) * p.ldo + static_cast<long>(hd[x]) * D + c2;
+          uint16_t *out = p.out + (w.q0 + tok0 + r / p.group) * p.ldo +
+                          static_cast<long>(w.h * p.group + r % p.group) * D + c2;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
             *reinterpret_cast<uint32_t *>(out + d * 8) =
                 pack2<F16>(o[d][2 * x] * inv, o[d][2 * x + 1] * inv);
-        }
-      } else {
-        const int slot = w.blk == 0;
-        float *ml = slot_ml(p, blockIdx.x, slot);
-        float *po = slot_o(p, blockIdx.x, slot);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = wm * 16 + g + 8 * x;
-          if (!row_ok[x]) continue;
+        } else {
           if ((lane & 3) == 0) {
             ml[r] = m[x];
             ml[p.rows + r] = l[x];
@@ -410,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     next_unit<kKeys>(p, w, e);
     // the piece that goes on is this CTA's last
     if (threadIdx.x == 0 && w.pos >= w.end && !goes_on) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    store_walk(w);
   }
   if (start->pos >= start->end && threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
   if (!ok && lane == 0) report_status(p.status, kStatusEpiWait);

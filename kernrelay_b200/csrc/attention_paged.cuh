@@ -198,14 +198,60 @@ __device__ __forceinline__ uint32_t visible32(const Params &p, const uint32_t *r
   return __funnelshift_r(lo, hi, j0 & 31) & there;
 }
 
-// Page of key block position `key` (a page outside the cache is reported and read as page 0).
-__device__ __forceinline__ int page_of(const Params &p, int b, int key) {
-  const int id = p.page_table[static_cast<long>(b) * p.ldp + (key >> p.page_shift)];
+// Entry `i` of sequence b's row of the page table (a page outside the cache is reported and read
+// as page 0).
+__device__ __forceinline__ int page_entry(const Params &p, int b, int i) {
+  const int id = p.page_table[static_cast<long>(b) * p.ldp + i];
   if (id < 0 || id >= p.pages) {
     report_status(p.status, kStatusBadIndex);
     return 0;
   }
   return id;
+}
+
+// The page numbers of a piece, in order, to a producer warp: a lane holds one of 32, and the next
+// 32 are on their way (under load a table entry takes as long as a block of keys).
+struct PageFeed {
+  int b, first, count;  // table row; first entry of the piece, entries
+  int at;               // entry (from `first`) of cur's lane 0
+  int cur, nxt;
+
+  __device__ __forceinline__ int load(const Params &p, int i) const {
+    return i < count ? page_entry(p, b, first + i) : 0;
+  }
+  // keys [key0, key1) of sequence b
+  __device__ __forceinline__ void begin(const Params &p, int b_, int key0, int key1) {
+    const int lane = threadIdx.x & 31;
+    b = b_;
+    first = key0 >> p.page_shift;
+    count = ((key1 - 1) >> p.page_shift) - first + 1;
+    at = 0;
+    cur = load(p, lane);
+    nxt = load(p, 32 + lane);
+  }
+  // the page of `key`, all lanes; keys of one call lie within 32 pages of the lowest, `low`, which
+  // never falls
+  __device__ __forceinline__ int page(const Params &p, int low, int key) {
+    if ((low >> p.page_shift) - first >= at + 32) {
+      at += 32;
+      cur = nxt;
+      nxt = load(p, at + 32 + (threadIdx.x & 31));
+    }
+    const int i = (key >> p.page_shift) - first - at;
+    const int a = __shfl_sync(0xffffffffu, cur, i & 31), c = __shfl_sync(0xffffffffu, nxt, i & 31);
+    return i < 32 ? a : c;
+  }
+};
+
+// Asks L2 for the page table while the schedule is searched: a line per thread of all CTAs.
+__device__ __forceinline__ void prefetch_page_table(const Params &p, int thread, int threads) {
+  const int lines = (p.max_pages + 31) / 32;  // of a row
+  const long i = static_cast<long>(blockIdx.x) * threads + thread;
+  if (i < static_cast<long>(lines) * p.B) {
+    const long row = i / lines;
+    const int32_t *at = p.page_table + row * p.ldp + (i - row * lines) * 32;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+  }
 }
 
 // What the combine kernel needs of a unit that CTA c starts and later CTAs go on with.

@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
     }
     fence_mbar_init();
   }
+  if (warp >= 2) prefetch_page_table(p, threadIdx.x - 64, C::kThreads - 64);
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
     constexpr int kHalves = D / 64;
     const int box = 1 << box_shift;
     const int bx = lane / kHalves, half = lane % kHalves;  // page 8 at D 128: 16 boxes x 2 halves
+    PageFeed feed;
     int n = 0, pieces = 0;
     bool ok = true;
     while (w.pos < w.end) {
@@ -244,6 +246,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
       const int end = kv_end(p, w.T, w.ctx, w.i);
       const int tok0 = w.i * p.tpt;
       const bool has_b = NT > 1 && tok0 + p.tile_tok < w.T;
+      feed.begin(p, w.b, w.blk * kKeys, min(end, e * kKeys));
       for (int a = 0; a < 2 * nblk && ok; ++a, ++n) {
         const bool is_v = a >= 2 && ((a & 1) == 0 || a == 2 * nblk - 1);
         const bool only = nblk == 1 && a == 1;  // one block: K0, V0
@@ -252,7 +255,8 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
         const int key0 = (w.blk + j) * kKeys;
         const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
         const int key = key0 + (bx << box_shift);
-        const int page = bx < nbox ? page_of(p, w.b, key) : 0;
+        // K of the next block comes before V of this one: the lower of the two sets the feed
+        const int page = feed.page(p, (w.blk + (v ? j : max(j - 1, 0))) * kKeys, key);
         const int s = n % C::kSlots;
         ok = mbar_wait(&empty[s], ((n / C::kSlots) & 1) ^ 1, kMbarLimitNs);
         if (a == 0 && ok) ok = mbar_wait(q_empty, (pieces & 1) ^ 1, kMbarLimitNs);
