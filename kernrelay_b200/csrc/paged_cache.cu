@@ -92,23 +92,30 @@ __device__ __forceinline__ uint4 ldg4(const void *p) {
   return __ldg(reinterpret_cast<const uint4 *>(p));
 }
 
-// One thread = 8 rotation pairs (elements j..j+7 and D/2+j..D/2+j+7) of one head of one token;
-// the D/16 threads of a head are neighbours in a warp and share its sum of squares.
+// One thread = 8 rotation pairs (elements j..j+7 and D/2+j..D/2+j+7) of one head of one token; the
+// D/16 threads of a head are neighbours in a warp and share its sum of squares.
 //   x^ = x * rsqrt(mean(x^2) + eps) * w;  y_lo = x_lo cos_lo - x_hi sin_lo,
 //   y_hi = x_hi cos_hi + x_lo sin_hi
 // in fp32 from the stored values to the one rounding of the store.
+//
+// Bound: HBM at size (every value read and written once), a launch when small.  What it takes is
+// loads in flight, and that is warps: the halves are rotated one after the other so that five CTAs
+// are resident (4 / 5 / 6 by the register limit: 48.8 / 44.2 / 45.6 us for 8192 tokens of 32 + 2 x 8
+// heads of 128 with norms, 203 MB, 31.6 us at the copy's rate; 8192 tokens of 14 + 2 x 2 heads of 64
+// 8.7 / 8.2 / 9.0).  Tried: several heads per warp with the table products in registers (54 us, 14.5),
+// and whole rows by bulk copies into shared memory (42.2 us, but 17.1).
 template <int D, bool F16>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
   constexpr int kLanes = HALF / 8;
-  const long gt = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int nh = a.HQ + 2 * a.HKV;
-  const long item = gt / kLanes;
+  const uint32_t gt = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t nh = a.HQ + 2 * a.HKV;
+  const uint32_t item = gt / kLanes;
   const int j = static_cast<int>(gt % kLanes) * 8;
-  if (item >= static_cast<long>(a.N) * nh) return;  // whole heads only
   const int n = static_cast<int>(item / nh);
-  const int h = static_cast<int>(item - static_cast<long>(n) * nh);
-  const uint16_t *p = a.qkv + n * a.ldqkv + static_cast<long>(h) * D + j;
+  if (n >= a.N) return;  // whole heads only
+  const int h = static_cast<int>(item - n * nh);
+  const uint16_t *p = a.qkv + n * a.ldqkv + h * D + j;
   // plain loads: q_out may be the q columns of qkv
   const uint4 wlo = *reinterpret_cast<const uint4 *>(p);
   const uint4 whi = *reinterpret_cast<const uint4 *>(p + HALF);
@@ -118,7 +125,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 
   uint16_t *dst;
   if (h < a.HQ) {
-    dst = a.q_out + n * a.ldq + static_cast<long>(h) * D + j;
+    dst = a.q_out + n * a.ldq + h * D + j;
   } else {
     const int64_t slot = a.slots[n];
     const bool slot_ok = slot >= 0 && slot < a.total_slots;
@@ -141,6 +148,9 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     *reinterpret_cast<uint4 *>(dst + HALF) = make_uint4(0, 0, 0, 0);
     return;
   }
+  const long t = pos * D + j;
+  const uint4 tc0 = ldg4(a.cos_tab + t), ts0 = ldg4(a.sin_tab + t);
+  const uint4 tc1 = ldg4(a.cos_tab + t + HALF), ts1 = ldg4(a.sin_tab + t + HALF);
   float lo[8], hi[8];
   unpack8<F16>(wlo, lo);
   unpack8<F16>(whi, hi);
@@ -154,27 +164,32 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
     const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-    float wl[8], wh[8];
-    unpack8<false>(ldg4(nw + j), wl);
-    unpack8<false>(ldg4(nw + HALF + j), wh);
+    float w[8];
+    unpack8<false>(ldg4(nw + j), w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] *= r * wl[e];
-      hi[e] *= r * wh[e];
-    }
+    for (int e = 0; e < 8; ++e) lo[e] *= r * w[e];
+    unpack8<false>(ldg4(nw + HALF + j), w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] *= r * w[e];
   }
-  const long t = pos * D + j;
   float c[8], s[8], y[8];
-  unpack8<false>(ldg4(a.cos_tab + t), c);
-  unpack8<false>(ldg4(a.sin_tab + t), s);
+  unpack8<false>(tc0, c);
+  unpack8<false>(ts0, s);
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = lo[e] * c[e] - hi[e] * s[e];
   *reinterpret_cast<uint4 *>(dst) = pack8<F16>(y);
-  unpack8<false>(ldg4(a.cos_tab + t + HALF), c);
-  unpack8<false>(ldg4(a.sin_tab + t + HALF), s);
+  unpack8<false>(tc1, c);
+  unpack8<false>(ts1, s);
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = hi[e] * c[e] + lo[e] * s[e];
   *reinterpret_cast<uint4 *>(dst + HALF) = pack8<F16>(y);
+}
+
+template <int D, bool F16>
+void launch_append(const AppendArgs &a, cudaStream_t stream) {
+  const long threads = static_cast<long>(a.N) * (a.HQ + 2 * a.HKV) * (D / 16);
+  if (threads > 0xffffff00L) throw CudaError("qk_norm_rope_paged: too many tokens");
+  append_kernel<D, F16><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(a);
 }
 
 // ------------------------------------------------------------------ page copies
@@ -229,18 +244,20 @@ struct CommitArgs {
 };
 
 // One CTA = one sequence and some of its (layer, K or V, head) rows.  It checks the sequence's
-// whole list first (so that a refused one is left whole), keeps the page and slot of source and
-// target in shared memory for kCommitChunk tokens at a time, and a thread moves one 16-byte
-// column: it reads the chunk's sources, then writes its targets.  accepted ascends strictly from
-// >= 0, so target i <= source i < later sources: no source is overwritten before it is read,
-// whatever the chunks.
+// whole list first (so that a refused one is left whole) and keeps page and slot of the moves in
+// shared memory, kCommitList at a time; a thread moves one 16-byte column, kCommitChunk moves at a
+// time: it reads their sources, then writes their targets.  accepted ascends strictly from >= 0,
+// so target i <= source i < later sources: no source is overwritten before it is read, whatever the
+// chunks.
 constexpr int kCommitThreads = 256;
 constexpr int kCommitChunk = 8;
+constexpr int kCommitList = 256;
 
 template <int D>
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
   constexpr int kLanes = D / 8;
   __shared__ int s_bad;
+  __shared__ int4 s_move[kCommitList];  // source page, slot; target page, slot (source page -1: stays)
   const int b = blockIdx.x;
   const int n = a.counts[b];
   const int64_t base = a.bases[b];
@@ -250,15 +267,24 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
   __syncthreads();
   const int32_t *acc = a.accepted + b * a.lda;
   const int32_t *table = a.page_table + b * a.ldp;
-  auto page_ok = [&](int64_t p) {
-    const int32_t id = table[p >> a.page_shift];
-    return id >= 0 && id < a.pages;
+  const int slot_mask = (1 << a.page_shift) - 1;
+  // move i of the list, checked
+  auto move = [&](int i, int4 &m) {
+    const int64_t x = acc[i];
+    const int64_t before = i ? acc[i - 1] : -1;
+    if (x <= before || base + x >= room) return false;
+    const int64_t from = base + x, to = base + i;
+    m = make_int4(table[from >> a.page_shift], static_cast<int>(from) & slot_mask,
+                  table[to >> a.page_shift], static_cast<int>(to) & slot_mask);
+    if (m.x < 0 || m.x >= a.pages || m.z < 0 || m.z >= a.pages) return false;
+    if (x == i) m.x = -1;
+    return true;
   };
   if (sizes_ok) {
     for (int i = threadIdx.x; i < n; i += kCommitThreads) {
-      const int64_t x = acc[i];
-      const int64_t before = i ? acc[i - 1] : -1;
-      if (x <= before || base + x >= room || !page_ok(base + x) || !page_ok(base + i)) s_bad = 1;
+      int4 m;
+      if (!move(i, m)) s_bad = 1;
+      else if (i < kCommitList) s_move[i] = m;
     }
   }
   __syncthreads();
@@ -268,25 +294,32 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
   }
   const int rows = a.layers * 2 * a.heads;
   const int row = blockIdx.y * (kCommitThreads / kLanes) + threadIdx.x / kLanes;
-  if (row >= rows) return;
   const int col = (threadIdx.x % kLanes) * 8;
   const int h = row % a.heads;
   const int kv = (row / a.heads) & 1;
   const int layer = row / (2 * a.heads);
-  uint16_t *mem = kv ? a.v + layer * a.v_layer + h * a.v_head : a.k + layer * a.k_layer + h * a.k_head;
+  uint16_t *mem = (kv ? a.v + layer * a.v_layer + h * a.v_head : a.k + layer * a.k_layer + h * a.k_head) + col;
   const long ps = kv ? a.v_page : a.k_page, ss = kv ? a.v_slot : a.k_slot;
-  auto at = [&](int64_t p) {
-    const long page = table[p >> a.page_shift];
-    return reinterpret_cast<uint4 *>(mem + page * ps + (p & ((1 << a.page_shift) - 1)) * ss + col);
-  };
-  for (int i0 = 0; i0 < n; i0 += kCommitChunk) {
-    uint4 w[kCommitChunk];
+  for (int l0 = 0; l0 < n; l0 += kCommitList) {
+    if (l0 > 0) {  // the next part of a long list
+      __syncthreads();
+      for (int i = l0 + threadIdx.x; i < min(n, l0 + kCommitList); i += kCommitThreads)
+        move(i, s_move[i - l0]);
+      __syncthreads();
+    }
+    if (row >= rows) continue;
+    const int m = min(n - l0, kCommitList);
+    for (int i0 = 0; i0 < m; i0 += kCommitChunk) {
+      uint4 w[kCommitChunk];
 #pragma unroll
-    for (int i = 0; i < kCommitChunk; ++i)
-      if (i0 + i < n && acc[i0 + i] != i0 + i) w[i] = *at(base + acc[i0 + i]);
+      for (int i = 0; i < kCommitChunk; ++i)
+        if (i0 + i < m && s_move[i0 + i].x >= 0)
+          w[i] = *reinterpret_cast<const uint4 *>(mem + s_move[i0 + i].x * ps + s_move[i0 + i].y * ss);
 #pragma unroll
-    for (int i = 0; i < kCommitChunk; ++i)
-      if (i0 + i < n && acc[i0 + i] != i0 + i) *at(base + i0 + i) = w[i];
+      for (int i = 0; i < kCommitChunk; ++i)
+        if (i0 + i < m && s_move[i0 + i].x >= 0)
+          *reinterpret_cast<uint4 *>(mem + s_move[i0 + i].z * ps + s_move[i0 + i].w * ss) = w[i];
+    }
   }
 }
 
@@ -340,14 +373,10 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
   a.total_slots = int64_t(c.pages) * c.page_size;
   a.eps = eps;
   a.status = status;
-  const long threads = static_cast<long>(N) * nh * (D / 16);
-  const long blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffL) throw CudaError("qk_norm_rope_paged: too many tokens");
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (D == 128 && c.dtype) append_kernel<128, true><<<g, 256, 0, stream>>>(a);
-  else if (D == 128) append_kernel<128, false><<<g, 256, 0, stream>>>(a);
-  else if (c.dtype) append_kernel<64, true><<<g, 256, 0, stream>>>(a);
-  else append_kernel<64, false><<<g, 256, 0, stream>>>(a);
+  if (D == 128 && c.dtype) launch_append<128, true>(a, stream);
+  else if (D == 128) launch_append<128, false>(a, stream);
+  else if (c.dtype) launch_append<64, true>(a, stream);
+  else launch_append<64, false>(a, stream);
   KRB_CUDA(cudaGetLastError());
 }
 
