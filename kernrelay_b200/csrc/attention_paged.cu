@@ -111,13 +111,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 4) {
     Walk w = *start;
-    // ---------------- producer: one TMA box per lane (page x half x K or V)
-    constexpr int kKinds = D / 64 * 2;
+    // ---------------- producer: one lane issues a stage's boxes (page x 64 columns, K and V).  A
+    // box per lane would be slower: TMA takes its operands from uniform registers, so the lanes'
+    // copies are issued one by one all the same, at 100 to 200 clocks each.
     const int box = 1 << box_shift;
-    const int bx = lane / kKinds, kind = lane % kKinds;
-    const bool is_v = kind >= D / 64;
-    const int half = kind % (D / 64);
-    const CUtensorMap *map = is_v ? &tm_v : &tm_k;
+    const uint32_t box_bytes = box * 128;
     PageFeed feed;
     int n = 0;  // blocks issued
     bool ok = true;
@@ -127,20 +125,29 @@ __global__ void __launch_bounds__(kThreads, 2)
       feed.begin(p, w.b, w.blk * kKeys, min(end, e * kKeys));
       for (int blk = w.blk; blk < e; ++blk, ++n) {
         const int s = n % C::kStages;
-        const int key = blk * kKeys + (bx << box_shift);
-        const int nbox = (min(kKeys, end - blk * kKeys) + box - 1) >> box_shift;
-        const int page = feed.page(p, blk * kKeys, key);
+        const int key0 = blk * kKeys;
+        const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
+        feed.advance(p, key0);
         ok = mbar_wait(&empty[s], ((n / C::kStages) & 1) ^ 1, kMbarLimitNs);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         uint8_t *stage = smem + s * 2 * C::kTile;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], nbox * box * 128 * kKinds);
-        __syncwarp();
-        if (bx < nbox)
-          tma_load_4d(stage + (is_v ? C::kTile : 0) + half * C::kHalf + (bx << box_shift) * 128,
-                      map, &full[s], half * 64, key & ((1 << p.page_shift) - 1), w.h, page);
+        const bool lead = elect_one();
+        if (lead) mbar_arrive_expect_tx(&full[s], nbox * box_bytes * (D / 64 * 2));
+        for (int i = 0; i < nbox; ++i) {
+          const int key = key0 + (i << box_shift);
+          const int page = feed.page(p, key), slot = key & ((1 << p.page_shift) - 1);
+          uint8_t *to = stage + i * box_bytes;
+          if (lead) {
+#pragma unroll
+            for (int half = 0; half < D / 64; ++half) {
+              tma_load_4d(to + half * C::kHalf, &tm_k, &full[s], half * 64, slot, w.h, page);
+              tma_load_4d(to + C::kTile + half * C::kHalf, &tm_v, &full[s], half * 64, slot, w.h, page);
+            }
+          }
+        }
       }
       if (ok) next_unit<kKeys>(p, w, e);
     }

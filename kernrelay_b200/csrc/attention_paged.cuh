@@ -229,19 +229,31 @@ struct PageFeed {
     cur = load(p, lane);
     nxt = load(p, 32 + lane);
   }
-  // the page of `key`, all lanes; keys of one call lie within 32 pages of the lowest, `low`, which
-  // never falls
-  __device__ __forceinline__ int page(const Params &p, int low, int key) {
+  // To be called before pages of keys from `low` on are asked for; `low` never falls.
+  __device__ __forceinline__ void advance(const Params &p, int low) {
     if ((low >> p.page_shift) - first >= at + 32) {
       at += 32;
       cur = nxt;
       nxt = load(p, at + 32 + (threadIdx.x & 31));
     }
+  }
+  // the page of `key` (the same for all lanes, within 32 pages of the last `low`)
+  __device__ __forceinline__ int page(const Params &p, int key) const {
     const int i = (key >> p.page_shift) - first - at;
-    const int a = __shfl_sync(0xffffffffu, cur, i & 31), c = __shfl_sync(0xffffffffu, nxt, i & 31);
-    return i < 32 ? a : c;
+    return __shfl_sync(0xffffffffu, i < 32 ? cur : nxt, i & 31);
   }
 };
+
+// one lane of a warp that is converged (the same one every time)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r != 0;
+}
 
 // Asks L2 for the page table while the schedule is searched: a line per thread of all CTAs.
 __device__ __forceinline__ void prefetch_page_table(const Params &p, int thread, int threads) {

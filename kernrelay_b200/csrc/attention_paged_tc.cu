@@ -2,15 +2,14 @@
 // chunks of a prompt): tcgen05 with S, P and O in TMEM.
 //
 // A unit is one or two 128-row tiles (whole tokens x the query heads of one KV head) that share
-// every K and V block; a block is 128 keys.  Per block and tile: S = Q K^T (SS form, both K-major),
-// the tile's 128 softmax threads (thread = row) turn S into P in place and O += P V (P from TMEM,
-// V from shared memory as it lies in the cache, [key][d], so MN-major: no transposed copy).
-// Issue order per block j: PV(A,j), QK(A,j+1), PV(B,j), QK(B,j+1), so one tile's products run
-// under the other tile's softmax.
+// every K and V block; a block is 64 keys.  Per block and tile: S = Q K^T (both operands K-major in
+// shared memory), the tile's 128 softmax threads (thread = row) turn S into P in place, and
+// O += P V (P from TMEM, V from shared memory as it lies in the cache, [key][d], so MN-major: no
+// transposed copy).  One warp issues all QK, another all PV, and a tile has two S / P stages in
+// TMEM: scores are a block ahead of the softmax, which never waits for the tensor pipe.
 //
-// Bound: with R rows the products take 4 R 128 D flop per block for 512 D bytes of K and V; from
-// about 250 rows on the softmax (128 x 128 exponentials per tile and block, 16 per clock and SM)
-// and the products bind, below it HBM does.
+// MEASURED
+//
 #include <algorithm>
 #include <string>
 
@@ -21,8 +20,10 @@ namespace paged {
 
 namespace {
 
-constexpr int kKeys = 128;
-constexpr uint32_t kChunk = 128 * 128;  // 128 rows x 64 elements, bytes
+constexpr int kKeys = 64;
+constexpr uint32_t kQChunk = 128 * 128;   // 128 query rows x 64 elements, bytes
+constexpr uint32_t kChunk = kKeys * 128;  // a block's keys x 64 elements, bytes
+constexpr int kSoftmaxWarp = 4;           // warps 0: Q and K, 3: V, 1: QK, 2: PV, 4 ..: softmax
 constexpr uint32_t kTmemCols = 512;
 // The running offset of a row moves (and O is rescaled) only when its maximum grew by more than
 // 2^8: until then P <= 256, which both 2-byte types hold with their full precision.
@@ -30,12 +31,13 @@ constexpr float kRescaleLog2 = 8.0f;
 
 template <int D, int NT>
 struct Cfg {
-  static constexpr int kTile = 256 * D;  // one Q tile, K block or V block, bytes
-  static constexpr int kSlots = D == 64 ? 8 : (NT == 2 ? 5 : 6);
-  static constexpr int kThreads = 64 + 128 * NT;
-  static constexpr int kBars = 2 * kSlots + 2 + 3 * NT;
+  static constexpr int kQTile = 256 * D;       // bytes
+  static constexpr int kTile = kKeys * D * 2;  // K or V block
+  static constexpr int kSlots = D == 64 ? 16 : (NT == 2 ? 10 : 12);
+  static constexpr int kThreads = 32 * kSoftmaxWarp + 128 * NT;
+  static constexpr int kBars = 2 * kSlots + 2 + 6 * NT;
   static constexpr int kSmem =
-      (NT + kSlots) * kTile + kBars * 8 + int(sizeof(Walk)) + 32 + 1024;
+      NT * kQTile + kSlots * kTile + kBars * 8 + int(sizeof(Walk)) + 32 + 1024;
 };
 
 // D[tmem] (+)= A[tmem] * B[smem], A 16-bit pairs K-major
@@ -69,6 +71,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
+      " %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -91,92 +107,94 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr) {
 __device__ __forceinline__ int k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int v_at(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * j + 1; }
 
-// One block of one row: S (128 columns at s_col) -> P over its first 64 columns, in one pass of
-// 32 scores at a time.  `see`(c): which of chunk c's 32 keys the row sees.  See attention_tc.cu's
-// softmax for the stale offset; here rows may have seen nothing yet (m = -inf), whose offset is 0.
-template <int D, bool F16, bool kMask, typename See>
-__device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, float scale_log2,
-                                              bool has_o, float &m_run, float &l_run, See see) {
-  float m_cur = m_run;
+// P = 2^(s * scale - off) of 64 scores, packed in the cache's type, and their sum in fp32.
+template <bool F16>
+__device__ __forceinline__ float exp_block(const uint32_t (&r)[2][32], float scale_log2, float off,
+                                          uint32_t (&pk)[32]) {
   float r8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  uint32_t ra[32], rb[32];
-  tmem_ld_32x32(s_col, ra);
-  tmem_wait_ld();
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t(&r)[32] = (c & 1) ? rb : ra;
-    if (c + 1 < 4) tmem_ld_32x32(s_col + (c + 1) * 32, (c & 1) ? ra : rb);
-    if constexpr (kMask) {
+  for (int e = 0; e < 32; ++e) {
+    const float p0 = exp2_mufu(fmaf(__uint_as_float(r[e >> 4][(2 * e) & 31]), scale_log2, -off));
+    const float p1 = exp2_mufu(fmaf(__uint_as_float(r[e >> 4][(2 * e + 1) & 31]), scale_log2, -off));
+    // P in the cache's type (its rounding is that of the output); the row sum takes the fp32 values
+    pk[e] = pack2<F16>(p0, p1);
+    r8[e & 7] += p0 + p1;
+  }
+  return ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
+}
+
+// A block of one row: S (64 columns at s_col) -> P over its first 32 columns.  `see`(c): which of
+// the 32 keys of half c the row sees.  P = 2^(s * scale - m) with the row's offset m, which moves
+// only by more than kRescaleLog2; O and l follow it.  The exponentials do not wait for the maximum:
+// they are taken with the old m, and once more where it moves (the first keys of a row, and
+// rarely after).  A row that has seen nothing yet has m = -inf and takes the offset 0.  `o_ready`
+// waits until no product writes O.
+template <int D, bool F16, bool kMask, typename See, typename Ready>
+__device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, float scale_log2,
+                                             bool has_o, float &m_run, float &l_run, See see,
+                                             Ready o_ready) {
+  uint32_t r[2][32];
+  tmem_ld_32x32(s_col, r[0]);
+  tmem_ld_32x32(s_col + 32, r[1]);
+  tmem_wait_ld();
+  if constexpr (kMask) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
       const uint32_t bits = see(c);
 #pragma unroll
       for (int e = 0; e < 32; ++e)
-        if (!((bits >> e) & 1)) r[e] = 0xff800000u;  // -inf
+        if (!((bits >> e) & 1)) r[c][e] = 0xff800000u;  // -inf
     }
-    float m8[8];
+  }
+  uint32_t pk[32];
+  float sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
+  float m8[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m8[e] = __uint_as_float(r[e]);
+  for (int e = 0; e < 8; ++e) m8[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
 #pragma unroll
-    for (int e = 8; e < 32; ++e) m8[e & 7] = fmaxf(m8[e & 7], __uint_as_float(r[e]));
-    const float cmax = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                             fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * scale_log2;
-    const bool grow = cmax - m_cur > kRescaleLog2;
-    if (c > 0 && __any_sync(0xffffffffu, grow)) {
-      // the P chunks of this block that are already written follow the new offset
-      const float f = grow ? exp2_mufu(m_cur - cmax) : 1.f;
-      tmem_wait_st();
+  for (int e = 8; e < 32; ++e)
+    m8[e & 7] = fmaxf(m8[e & 7], fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e])));
+  const float top = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                          fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * scale_log2;
+  const bool grow = top - m_run > kRescaleLog2;
+  if (__any_sync(0xffffffffu, grow)) {
+    const float alpha = grow ? exp2_mufu(m_run - top) : 1.f;
+    if (grow) m_run = top;
+    sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
+    l_run *= alpha;
+    if (has_o) {
+      o_ready();
 #pragma unroll 1
-      for (int pc = 0; pc < c; ++pc) {
-        uint32_t q[16];
-        tmem_ld16(s_col + pc * 16, q);
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld16(o_col + c * 16, o);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 pr = unpack2<F16>(q[e]);
-          q[e] = pack2<F16>(pr.x * f, pr.y * f);
-        }
-        tmem_st16(s_col + pc * 16, q);
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+        tmem_st16(o_col + c * 16, o);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r8[e] *= f;
     }
-    if (grow) m_cur = cmax;
-    const float off = m_cur == -INFINITY ? 0.f : m_cur;
-    uint32_t pk[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p0 = exp2_mufu(fmaf(__uint_as_float(r[2 * e]), scale_log2, -off));
-      const float p1 = exp2_mufu(fmaf(__uint_as_float(r[2 * e + 1]), scale_log2, -off));
-      // P in the cache's type; the row sum takes the fp32 values
-      pk[e] = pack2<F16>(p0, p1);
-      r8[e & 7] += p0 + p1;
-    }
-    tmem_st16(s_col + c * 16, pk);
-    if (c + 1 < 4) tmem_wait_ld();
   }
+  l_run += sum;
+  tmem_st32(s_col, pk);
   tmem_wait_st();
-  const float rs = ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
-  const bool moved = m_cur != m_run;
-  const float alpha = moved ? exp2_mufu(m_run - m_cur) : 1.f;
-  if (has_o && __any_sync(0xffffffffu, moved)) {
-#pragma unroll 1
-    for (int c = 0; c < D / 16; ++c) {
-      uint32_t r[16];
-      tmem_ld16(o_col + c * 16, r);
-      tmem_wait_ld();
+}
+
+// 64 bytes of this thread's row (null: it has none)
+__device__ __forceinline__ void store_rows(uint8_t *dst, const uint32_t (&v)[16]) {
+  if (!dst) return;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
-      tmem_st16(o_col + c * 16, r);
-    }
-    tmem_wait_st();
-  }
-  l_run = l_run * alpha + rs;
-  m_run = m_cur;
+  for (int q = 0; q < 16; q += 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 4 * q), "r"(v[q]),
+                 "r"(v[q + 1]), "r"(v[q + 2]), "r"(v[q + 3]), "r"(v[q + 4]), "r"(v[q + 5]), "r"(v[q + 6]),
+                 "r"(v[q + 7])
+                 : "memory");
 }
 
 }  // namespace
 
 template <int D, int NT, bool F16>
-__global__ void __launch_bounds__(64 + 128 * NT, 1)
+__global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
     attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q,
                          const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const Params p, int box_shift) {
@@ -184,15 +202,15 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem =
       reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *ring = smem + NT * C::kTile;
+  uint8_t *ring = smem + NT * C::kQTile;
   uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::kSlots * C::kTile);
   uint64_t *empty = full + C::kSlots;
   uint64_t *q_full = empty + C::kSlots;
   uint64_t *q_empty = q_full + 1;
-  uint64_t *s_full = q_empty + 1;
-  uint64_t *p_ready = s_full + NT;
-  uint64_t *o_done = p_ready + NT;
-  Walk *start = reinterpret_cast<Walk *>(o_done + NT);
+  uint64_t *s_full = q_empty + 1;       // [tile][stage], like the next two
+  uint64_t *p_ready = s_full + 2 * NT;
+  uint64_t *o_done = p_ready + 2 * NT;  // PV of the stage's P
+  Walk *start = reinterpret_cast<Walk *>(o_done + 2 * NT);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(start + 1);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -205,7 +223,7 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int i = 0; i < NT; ++i) {
+    for (int i = 0; i < 2 * NT; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 128);
       mbar_init(&o_done[i], 1);
@@ -232,151 +250,185 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
   const uint32_t tmem = *tmem_slot;
   Walk w = *start;
 
-  if (warp == 0) {
-    // ---------------- TMA producer: a box (page x 64 columns) per lane
-    constexpr int kHalves = D / 64;
+  if (warp == 0 || warp == 3) {
+    // ---------------- producers: warp 0 brings Q and K, warp 3 V; one lane issues the boxes (page x
+    // 64 columns).  TMA takes its operands from uniform registers: boxes of several lanes would be
+    // issued one by one all the same, at 100 to 200 clocks each.
+    const bool v = warp == 3;
     const int box = 1 << box_shift;
-    const int bx = lane / kHalves, half = lane % kHalves;  // page 8 at D 128: 16 boxes x 2 halves
+    const uint32_t box_bytes = box * 128;
     PageFeed feed;
-    int n = 0, pieces = 0;
+    int base = 0, pieces = 0;  // ring index of the piece's first load
+    int last = -1;             // ring index of this warp's last load
     bool ok = true;
     while (w.pos < w.end) {
       const int e = piece_end(w);
       const int nblk = e - w.blk;
       const int end = kv_end(p, w.T, w.ctx, w.i);
       const int tok0 = w.i * p.tpt;
-      const bool has_b = NT > 1 && tok0 + p.tile_tok < w.T;
       feed.begin(p, w.b, w.blk * kKeys, min(end, e * kKeys));
-      for (int a = 0; a < 2 * nblk && ok; ++a, ++n) {
-        const bool is_v = a >= 2 && ((a & 1) == 0 || a == 2 * nblk - 1);
-        const bool only = nblk == 1 && a == 1;  // one block: K0, V0
-        const bool v = is_v || only;
-        const int j = v ? (a == 2 * nblk - 1 ? nblk - 1 : a / 2 - 1) : (a + 1) / 2;
-        const int key0 = (w.blk + j) * kKeys;
-        const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
-        const int key = key0 + (bx << box_shift);
-        // K of the next block comes before V of this one: the lower of the two sets the feed
-        const int page = feed.page(p, (w.blk + (v ? j : max(j - 1, 0))) * kKeys, key);
-        const int s = n % C::kSlots;
-        ok = mbar_wait(&empty[s], ((n / C::kSlots) & 1) ^ 1, kMbarLimitNs);
-        if (a == 0 && ok) ok = mbar_wait(q_empty, (pieces & 1) ^ 1, kMbarLimitNs);
+      if (!v) {
+        const bool has_b = NT > 1 && tok0 + p.tile_tok < w.T;
+        ok = mbar_wait(q_empty, (pieces & 1) ^ 1, kMbarLimitNs);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint8_t *dst = ring + s * C::kTile;
-        if (lane == 0) {
-          if (a == 0) {
-            const uint32_t bytes = p.tile_tok * p.group * D * 2;
-            mbar_arrive_expect_tx(q_full, has_b ? 2 * bytes : bytes);
+        if (elect_one()) {
+          const uint32_t bytes = p.tile_tok * p.group * D * 2;
+          mbar_arrive_expect_tx(q_full, has_b ? 2 * bytes : bytes);
+          for (int x = 0; x < (has_b ? 2 : 1); ++x)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-              if (x && !has_b) break;
-#pragma unroll
-              for (int c = 0; c < kHalves; ++c)
-                tma_load_4d(smem + x * C::kTile + c * kChunk, &tm_q, q_full, 64 * c, w.h * p.group,
-                            w.q0 + tok0 + x * p.tile_tok, 0);
-            }
-          }
-          mbar_arrive_expect_tx(&full[s], nbox * box * 128 * kHalves);
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(smem + x * C::kQTile + c * kQChunk, &tm_q, q_full, 64 * c, w.h * p.group,
+                          w.q0 + tok0 + x * p.tile_tok, 0);
         }
-        __syncwarp();
-        if (bx < nbox)
-          tma_load_4d(dst + half * kChunk + (bx << box_shift) * 128, v ? &tm_v : &tm_k, &full[s],
-                      half * 64, key & ((1 << p.page_shift) - 1), w.h, page);
+      }
+      for (int j = 0; j < nblk; ++j) {
+        const int at = base + (v ? v_at(j, nblk) : k_at(j));
+        const int s = at % C::kSlots;
+        const int key0 = (w.blk + j) * kKeys;
+        const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
+        feed.advance(p, key0);
+        ok = mbar_wait(&empty[s], ((at / C::kSlots) & 1) ^ 1, kMbarLimitNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const bool lead = elect_one();
+        if (lead) mbar_arrive_expect_tx(&full[s], nbox * box_bytes * (D / 64));
+        const CUtensorMap *map = v ? &tm_v : &tm_k;
+        for (int i = 0; i < nbox; ++i) {
+          const int key = key0 + (i << box_shift);
+          const int page = feed.page(p, key), slot = key & ((1 << p.page_shift) - 1);
+          if (lead) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(ring + s * C::kTile + c * kChunk + i * box_bytes, map, &full[s], 64 * c, slot,
+                          w.h, page);
+          }
+        }
+        last = at;
       }
       if (!ok) break;
+      base += 2 * nblk;
       ++pieces;
       next_unit<kKeys>(p, w, e);
     }
     if (!ok && lane == 0) report_status(p.status, kStatusTmaWait);
-    // no TMA write may still be in flight when the CTA exits
-    for (int i = max(0, n - C::kSlots); i < n; ++i)
-      mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, kMbarLimitNs / 4);
-    if (pieces) mbar_wait(q_full, (pieces - 1) & 1, kMbarLimitNs / 4);
+    // No TMA write may still be in flight when the CTA exits.  Every load is waited for by an issuer;
+    // after a wait that ran out, give this warp's own (a slot has been given back only when its load
+    // was complete, so a phase that is not there any more costs the limit and no more).
+    if (!ok && last >= 0)
+      for (int i = max(0, last - C::kSlots + 1); i <= last; ++i)
+        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, kMbarLimitNs / 64);
+    if (!ok && !v && pieces) mbar_wait(q_full, (pieces - 1) & 1, kMbarLimitNs / 64);
   } else if (warp == 1) {
+    // ---------------- QK issuer (one thread)
     if (lane == 0) {
-      // ---------------- MMA issuer
-      constexpr uint32_t idesc_s = F16 ? idesc_f16_f32(128, 128) : idesc_bf16_f32(128, 128);
-      // B (V) MN-major: bit 16
-      constexpr uint32_t idesc_o = (F16 ? idesc_f16_f32(128, D) : idesc_bf16_f32(128, D)) | (1u << 16);
+      constexpr uint32_t idesc = F16 ? idesc_f16_f32(128, kKeys) : idesc_bf16_f32(128, kKeys);
       const uint64_t dq = sdesc_kmajor_sw128(smem_u32(smem));
       const uint64_t dk = sdesc_kmajor_sw128(smem_u32(ring));
-      const uint64_t dv = sdesc_mnmajor_sw128(smem_u32(ring));
-      constexpr uint64_t kTile16 = C::kTile >> 4;
-      int base = 0, pieces = 0;  // ring index of the piece's first load
+      int base = 0, pieces = 0;   // ring index of the piece's first load; pieces
       uint32_t done[2] = {0, 0};  // blocks of each tile so far (a piece may lack the second)
       bool ok = true;
-      auto wait_full = [&](int at) {
-        return mbar_wait(&full[at % C::kSlots], (at / C::kSlots) & 1, kMbarLimitNs);
-      };
-      auto issue_qk = [&](int x, int at) {
-        tc_fence_after();
-        const uint64_t q = dq + x * kTile16, k = dk + (at % C::kSlots) * kTile16;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          // 16 columns of D per step, 64 per chunk
-          const uint64_t step = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
-          umma_bf16(tmem + 256 * x, q + step, k + step, idesc_s, kk > 0);
-        }
-        umma_commit(&s_full[x]);
-      };
       while (w.pos < w.end && ok) {
         const int e = piece_end(w);
-        const int nblk = e - w.blk;
+        const int n = e - w.blk;
         const int nx = NT > 1 && w.i * p.tpt + p.tile_tok < w.T ? 2 : 1;
-        ok = mbar_wait(q_full, pieces & 1, kMbarLimitNs) && wait_full(base);
-        if (!ok) break;
-        for (int x = 0; x < nx; ++x) issue_qk(x, base);
-        umma_commit(&empty[base % C::kSlots]);
-        if (nblk == 1) umma_commit(q_empty);
-        for (int j = 0; j < nblk && ok; ++j) {
-          const int vat = base + v_at(j, nblk), kat = base + k_at(j + 1);
-          const bool more = j + 1 < nblk;
-          for (int x = 0; x < nx; ++x) {
-            const uint32_t par = done[x]++ & 1;
-            ok = mbar_wait(&p_ready[x], par, kMbarLimitNs);
-            if (ok && x == 0) ok = wait_full(vat);
+        ok = mbar_wait(q_full, pieces & 1, kMbarLimitNs);
+        for (int j = 0; j < n && ok; ++j) {
+          const int at = (base + k_at(j)) % C::kSlots;
+          ok = mbar_wait(&full[at], ((base + k_at(j)) / C::kSlots) & 1, kMbarLimitNs);
+          const uint64_t k = dk + at * (C::kTile >> 4);
+          for (int x = 0; x < nx && ok; ++x) {
+            const uint32_t c = done[x]++, stage = c & 1;
+            // S overwrites the P of the tile's block before last
+            if (c >= 2) ok = mbar_wait(&o_done[2 * x + stage], ((c >> 1) - 1) & 1, kMbarLimitNs);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t v = dv + (vat % C::kSlots) * kTile16;
+            const uint64_t q = dq + ((x * C::kQTile) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys per step
-              umma_ts(tmem + 256 * x + 128, tmem + 256 * x + kk * 8, v + ((kk * 2048) >> 4), idesc_o,
-                      j > 0 || kk > 0);
-            umma_commit(&o_done[x]);
-            if (x == nx - 1) umma_commit(&empty[vat % C::kSlots]);
-            // QK(x, j+1) overwrites P(x, j); the next piece's first one does, too
-            ok = mbar_wait(&o_done[x], par, kMbarLimitNs);
-            if (ok && more && x == 0) ok = wait_full(kat);
-            if (!ok) break;
-            if (more) {
-              issue_qk(x, kat);
-              if (x == nx - 1) {
-                umma_commit(&empty[kat % C::kSlots]);
-                if (j + 2 == nblk) umma_commit(q_empty);
-              }
-            }
+            for (int kk = 0; kk < D / 16; ++kk)  // 16 columns of D per step, 64 per chunk
+              umma_bf16(tmem + 256 * x + 64 * stage, q + (((kk >> 2) * kQChunk + (kk & 3) * 32) >> 4),
+                        k + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4), idesc, kk > 0);
+            umma_commit(&s_full[2 * x + stage]);
           }
+          if (ok) umma_commit(&empty[at]);
         }
-        base += 2 * nblk;
+        if (ok) umma_commit(q_empty);
+        base += 2 * n;
         ++pieces;
         next_unit<kKeys>(p, w, e);
       }
       if (!ok) report_status(p.status, kStatusMmaWait);
     }
-  } else {
+  } else if (warp == 2) {
+    // ---------------- PV issuer (lane 0; the other lanes keep step: they zero the rows of V behind
+    // the last key)
+    constexpr uint32_t idesc =
+        (F16 ? idesc_f16_f32(128, D) : idesc_bf16_f32(128, D)) | (1u << 16);  // B (V) MN-major
+    const uint64_t dv = sdesc_mnmajor_sw128(smem_u32(ring));
+    int base = 0;
+    uint32_t done[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      ok = mbar_wait(bar, parity, kMbarLimitNs);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    while (w.pos < w.end && ok) {
+      const int e = piece_end(w);
+      const int n = e - w.blk;
+      const int end = kv_end(p, w.T, w.ctx, w.i);
+      const int nx = NT > 1 && w.i * p.tpt + p.tile_tok < w.T ? 2 : 1;
+      for (int j = 0; j < n; ++j) {
+        const int at = (base + v_at(j, n)) % C::kSlots;
+        const int z0 = end - (w.blk + j) * kKeys;  // keys of the block that are there
+        if (!wait(&full[at], ((base + v_at(j, n)) / C::kSlots) & 1)) break;
+        if (z0 < kKeys) {
+          // V rows behind the last key may be anything (stale or never written memory, whose
+          // infinities a zero probability would not cancel): zero them
+          const uint32_t vt = smem_u32(ring + at * C::kTile);
+          for (int u = lane; u < (kKeys - z0) * (D / 8); u += 32) {
+            const int key = z0 + u / (D / 8), c16 = u % (D / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             vt + (c16 >> 3) * kChunk + key * 128 + (c16 & 7) * 16),
+                         "r"(0)
+                         : "memory");
+          }
+          fence_proxy_async_shared();
+          __syncwarp();
+        }
+        const uint64_t v = dv + at * (C::kTile >> 4);
+        for (int x = 0; x < nx; ++x) {
+          const uint32_t c = done[x]++, stage = c & 1;
+          if (!wait(&p_ready[2 * x + stage], (c >> 1) & 1)) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys (8 columns of P) per step
+              umma_ts(tmem + 256 * x + 128, tmem + 256 * x + 64 * stage + kk * 8,
+                      v + ((kk * 2048) >> 4), idesc, j > 0 || kk > 0);
+            umma_commit(&o_done[2 * x + stage]);
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) umma_commit(&empty[at]);
+      }
+      base += 2 * n;
+      next_unit<kKeys>(p, w, e);
+    }
+    if (!ok && lane == 0) report_status(p.status, kStatusMmaWait);
+  } else if (warp >= kSoftmaxWarp) {
     // ---------------- softmax, epilogue: 128 threads per tile, thread = row
-    const int x = (warp - 2) >> 2;
+    const int x = (warp - kSoftmaxWarp) >> 2;
     const int quad = warp & 3;  // TMEM lane quadrant of this warp
     const int row = quad * 32 + lane;
     const uint32_t s_col = tmem + (static_cast<uint32_t>(quad * 32) << 16) + 256 * x;
     const uint32_t o_col = s_col + 128;
     const int rt = row / p.group, rg = row - rt * p.group;
-    int base = 0, mine = 0;  // ring index of the piece's first load; blocks of this tile so far
+    int mine = 0;  // blocks of this tile so far
     bool ok = true;
     while (w.pos < w.end) {
       const int e = piece_end(w);
       const int nblk = e - w.blk;
-      const int end = kv_end(p, w.T, w.ctx, w.i);
       const int tok0 = w.i * p.tpt + x * p.tile_tok;
       const int ntok = min(p.tile_tok, w.T - tok0);
       if (ntok > 0) {
@@ -388,43 +440,32 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
         float m_run = -INFINITY, l_run = 0.f;
         for (int j = 0; j < nblk && ok; ++j) {
           const int key0 = (w.blk + j) * kKeys;
-          ok = mbar_wait(&s_full[x], (mine + j) & 1, kMbarLimitNs);
+          const int c = mine + j, stage = c & 1;  // blocks of this tile before this one
+          ok = mbar_wait(&s_full[2 * x + stage], (c >> 1) & 1, kMbarLimitNs);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_fence_after();
           if (any_row) {
+            // PV of the block before (that of the one before it is complete: this S came after it)
+            auto o_ready = [&] {
+              if (!mbar_wait(&o_done[2 * x + (stage ^ 1)], ((c - 1) >> 1) & 1, kMbarLimitNs)) ok = false;
+              tc_fence_after();
+            };
             if (key0 + kKeys > hidden_from)
-              softmax_block<D, F16, true>(s_col, o_col, p.scale_log2, j > 0, m_run, l_run, [&](int c) {
-                return visible32(p, row_mask, w.T, t, key0 + c * 32 - w.ctx);
-              });
+              softmax_block<D, F16, true>(
+                  s_col + 64 * stage, o_col, p.scale_log2, j > 0, m_run, l_run,
+                  [&](int q) { return visible32(p, row_mask, w.T, t, key0 + q * 32 - w.ctx); }, o_ready);
             else
-              softmax_block<D, F16, false>(s_col, o_col, p.scale_log2, j > 0, m_run, l_run,
-                                           [](int) { return 0u; });
-          }
-          if (x == 0 && key0 + kKeys > end) {
-            // V rows behind the last key may be anything (stale or never written memory, whose
-            // infinities a zero probability would not cancel): zero them before PV reads them
-            const int at = base + v_at(j, nblk);
-            ok = mbar_wait(&full[at % C::kSlots], (at / C::kSlots) & 1, kMbarLimitNs);
-            const int z0 = end - key0;
-            const uint32_t vt = smem_u32(ring + (at % C::kSlots) * C::kTile);
-            if (ok)
-              for (int u = row; u < (kKeys - z0) * (D / 8); u += 128) {
-                const int key = z0 + u / (D / 8), c16 = u % (D / 8);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                 vt + (c16 >> 3) * kChunk + key * 128 + (c16 & 7) * 16),
-                             "r"(0)
-                             : "memory");
-              }
-            fence_proxy_async_shared();
+              softmax_block<D, F16, false>(s_col + 64 * stage, o_col, p.scale_log2, j > 0, m_run, l_run,
+                                           [](int) { return 0u; }, o_ready);
           }
           tc_fence_before();
-          mbar_arrive(&p_ready[x]);
+          mbar_arrive(&p_ready[2 * x + stage]);
         }
         mine += nblk;
-        if (ok) ok = mbar_wait(&o_done[x], (mine - 1) & 1, kMbarLimitNs);
+        if (ok) ok = mbar_wait(&o_done[2 * x + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, kMbarLimitNs);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -432,49 +473,45 @@ __global__ void __launch_bounds__(64 + 128 * NT, 1)
         tc_fence_after();
         if (any_row) {
           const bool whole = w.blk == 0 && e == w.nblk;
-          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-          uint16_t *out = p.out + (w.q0 + t) * p.ldo + static_cast<long>(w.h * p.group + rg) * D;
-          const int slot = w.blk == 0, sr = x * 128 + row;
-          float *po = slot_o(p, blockIdx.x, slot) + static_cast<long>(sr) * D;
-          if (!whole && row_ok) {
-            float *ml = slot_ml(p, blockIdx.x, slot);
-            ml[sr] = m_run;
-            ml[p.rows + sr] = l_run;
-          }
+          if (whole) {
+            const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+            uint16_t *out = p.out + (w.q0 + t) * p.ldo + static_cast<long>(w.h * p.group + rg) * D;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32(o_col + c * 32, r);
-            tmem_wait_ld();
-            if (row_ok && whole) {
-              uint4 *o4 = reinterpret_cast<uint4 *>(out + c * 32);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32], v[16];
+              tmem_ld_32x32(o_col + c * 32, r);
+              tmem_wait_ld();
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint4 v;
-                v.x = pack2<F16>(__uint_as_float(r[q * 8 + 0]) * inv, __uint_as_float(r[q * 8 + 1]) * inv);
-                v.y = pack2<F16>(__uint_as_float(r[q * 8 + 2]) * inv, __uint_as_float(r[q * 8 + 3]) * inv);
-                v.z = pack2<F16>(__uint_as_float(r[q * 8 + 4]) * inv, __uint_as_float(r[q * 8 + 5]) * inv);
-                v.w = pack2<F16>(__uint_as_float(r[q * 8 + 6]) * inv, __uint_as_float(r[q * 8 + 7]) * inv);
-                o4[q] = v;
-              }
-            } else if (row_ok) {
-              uint4 *o4 = reinterpret_cast<uint4 *>(po + c * 32);
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                o4[q] = make_uint4(r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]);
+              for (int q = 0; q < 16; ++q)
+                v[q] = pack2<F16>(__uint_as_float(r[2 * q]) * inv, __uint_as_float(r[2 * q + 1]) * inv);
+              store_rows(row_ok ? reinterpret_cast<uint8_t *>(out + c * 32) : nullptr, v);
+            }
+          } else {
+            const int slot = w.blk == 0, sr = x * 128 + row;
+            float *po = slot_o(p, blockIdx.x, slot) + static_cast<long>(sr) * D;
+            if (row_ok) {
+              float *ml = slot_ml(p, blockIdx.x, slot);
+              ml[sr] = m_run;
+              ml[p.rows + sr] = l_run;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              tmem_ld16(o_col + c * 16, v);
+              tmem_wait_ld();
+              store_rows(row_ok ? reinterpret_cast<uint8_t *>(po + c * 16) : nullptr, v);
             }
           }
         }
       }
-      base += 2 * nblk;
       const bool goes_on = w.blk == 0 && e < w.nblk;
-      if (threadIdx.x == 64 && goes_on) p.desc[blockIdx.x] = split_desc(p, w);
+      if (threadIdx.x == 32 * kSoftmaxWarp && goes_on) p.desc[blockIdx.x] = split_desc(p, w);
       next_unit<kKeys>(p, w, e);
       // the piece that goes on is this CTA's last
-      if (threadIdx.x == 64 && w.pos >= w.end && !goes_on)
+      if (threadIdx.x == 32 * kSoftmaxWarp && w.pos >= w.end && !goes_on)
         p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
-    if (threadIdx.x == 64 && (start->pos >= start->end || !ok))
+    if (threadIdx.x == 32 * kSoftmaxWarp && (start->pos >= start->end || !ok))
       p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (!ok && lane == 0) report_status(p.status, kStatusEpiWait);
   }
