@@ -1,12 +1,13 @@
 // Attention of new tokens over the paged K/V cache: the form for few query rows (a token or a
 // small draft per sequence) on mma.sync, the kernel that joins split units, and the host side.
 //
-// Few rows are bound by reading K and V once: a 64-key block of one KV head is 32 KB at
-// head_dim 128 and feeds 4 * rows * 64 * 128 flop, 1 us of one SM's share of HBM bandwidth for
-// 0.13 us of tensor work at 16 rows.  So the kernel is a deep ring of TMA loads (two CTAs of three
-// 32 KB stages per SM, about twice the bytes that latency needs in flight) and the rows of all
-// query heads that share a KV head go through the tensor cores together.  mma.sync takes 16-row
-// tiles, so 7 rows of a decoded token cost one of them; tcgen05 would pad them to 64 or 128.
+// Few rows are bound by reading K and V once: a 64-key block of one KV head is 32 KB at head_dim 128,
+// 0.75 us of one SM's share of HBM bandwidth, against 0.14 us of mma.sync for a 16-row tile.  So the
+// kernel is a ring of TMA loads (two CTAs of three 32 KB stages per SM, three times the bytes that
+// latency needs in flight), the rows of all query heads that share a KV head go through the tensor
+// cores together, and the four warps of a CTA split the keys, so that a block costs each a quarter.
+// Measured: 64 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads of 128,
+// 111 us, 92 % of what 659 MB take at the copy's rate; 2 sequences of 98 and 131 thousand, 80 us, 91 %.
 #include <algorithm>
 #include <string>
 
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint32_t tile_off(int key, int chunk) {
 
 }  // namespace
 
-// Warp (wm, wn) of the WM x (4 / WM) consumer warps: rows 16 wm .. +15 of the unit, keys
+// Warp (wm, wn) of the WM x (4 / WM) consumer warps (WM 1 or 2): rows 16 wm .. +15 of the unit, keys
 // wn * 16 WM .. of every block.  A lane holds rows g = lane / 4 and g + 8 (mma fragments).
 template <int D, int WM, bool F16>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -441,43 +442,41 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ------------------------------------------------------------------ joining split units
-// CTA (c, y) joins rows y * 4 / KW .. of the unit that CTA c of the attention kernel began and later
-// ones went on with: KW warps per row, each every KW-th piece, then their sums in order;
-// O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.  A long sequence over few units is cut into
-// dozens of pieces (KW = 4: few rows), a wide draft into two or three (KW = 1).
-template <int D, int KW, bool F16>
+// CTA (c, r) joins row r of the unit that CTA c of the attention kernel began and later ones went on
+// with: each of its warps takes every fourth piece (a long sequence over few units is cut into
+// dozens; one warp alone took 12 us for 37 pieces), then their sums in order;
+// O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+template <int D, bool F16>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   constexpr int V = D / 32;  // columns of a lane
-  constexpr int kUnroll = 4;
-  __shared__ float part[4][32][V + 1];
+  constexpr int KW = 4, kUnroll = 4;
+  __shared__ float part[KW][32][V + 1];
   pdl_wait();
   const int c = blockIdx.x;
   const int4 d = p.desc[c];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = (blockIdx.y * 4 + warp) / KW, kw = warp % KW;
-  if (d.w < 2 || (blockIdx.y * 4) / KW >= d.y * p.group) return;
-  const bool row_ok = r < d.y * p.group;
+  const int r = blockIdx.y;
+  if (d.w < 2 || r >= d.y * p.group) return;
   const int tok = r / p.group, g = r - tok * p.group;
-  const int sr = row_ok ? slot_row(p, tok, g) : 0;
-  const int pieces = row_ok ? d.w : 0;
+  const int pieces = d.w;
   float mx = -INFINITY;
-  for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, slot_ml(p, c + k, k == 0)[sr]);
+  for (int k = lane; k < pieces; k += 32) mx = fmaxf(mx, slot_ml(p, c + k, k == 0)[r]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float off = mx == -INFINITY ? 0.f : mx;
   float total = 0.f, acc[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) acc[x] = 0.f;
-  for (int k0 = kw; k0 < pieces; k0 += KW * kUnroll) {
+  for (int k0 = warp; k0 < pieces; k0 += KW * kUnroll) {
     float f[kUnroll], l[kUnroll], v[kUnroll][V];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int k = k0 + u * KW;
       if (k >= pieces) continue;
       const float *ml = slot_ml(p, c + k, k == 0);
-      f[u] = ml[sr];
-      l[u] = ml[p.rows + sr];
-      const float *o = slot_o(p, c + k, k == 0) + static_cast<long>(sr) * D + lane * V;
+      f[u] = ml[r];
+      l[u] = ml[p.rows + r];
+      const float *o = slot_o(p, c + k, k == 0) + static_cast<long>(r) * D + lane * V;
       if constexpr (V == 4) {
         const float4 t = *reinterpret_cast<const float4 *>(o);
         v[u][0] = t.x, v[u][1] = t.y, v[u][2] = t.z, v[u][3] = t.w;
@@ -495,20 +494,17 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
       for (int x = 0; x < V; ++x) acc[x] += w * v[u][x];
     }
   }
-  if constexpr (KW > 1) {
 #pragma unroll
-    for (int x = 0; x < V; ++x) part[warp][lane][x] = acc[x];
-    part[warp][lane][V] = total;
-    __syncthreads();
-    if (kw != 0) return;
+  for (int x = 0; x < V; ++x) part[warp][lane][x] = acc[x];
+  part[warp][lane][V] = total;
+  __syncthreads();
+  if (warp != 0) return;
 #pragma unroll
-    for (int k = 1; k < KW; ++k) {
+  for (int k = 1; k < KW; ++k) {
 #pragma unroll
-      for (int x = 0; x < V; ++x) acc[x] += part[warp + k][lane][x];
-      total += part[warp + k][lane][V];
-    }
+    for (int x = 0; x < V; ++x) acc[x] += part[k][lane][x];
+    total += part[k][lane][V];
   }
-  if (!row_ok) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   uint16_t *out = p.out + (d.x + tok) * p.ldo + static_cast<long>(d.z * p.group + g) * D + lane * V;
   if constexpr (V == 4)
@@ -519,11 +515,9 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ host side
-template <int KW>
-static void combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
-  const int rows = std::min(p.tpt, p.max_q) * p.group;
+void launch_dependent(void (*kern)(const Params), dim3 grid, const Params &p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, (rows * KW + 3) / 4);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -531,14 +525,13 @@ static void combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, KW, true> : combine_kernel<128, KW, false>)
-                          : (f16 ? combine_kernel<64, KW, true> : combine_kernel<64, KW, false>);
   KRB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 static void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
-  if (p.rows <= 16) combine<4>(p, ctas, f16, stream);
-  else combine<1>(p, ctas, f16, stream);
+  auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, true> : combine_kernel<128, false>)
+                          : (f16 ? combine_kernel<64, true> : combine_kernel<64, false>);
+  launch_dependent(kern, dim3(ctas, std::min(p.tpt, p.max_q) * p.group), p, stream);
 }
 
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys) {
@@ -591,9 +584,9 @@ static void launch(const Params &p, const KvMaps &maps, int ctas, int device, cu
 template <int D, bool F16>
 static void launch_wm(int wm, const Params &p, const KvMaps &maps, int ctas, int device,
                       cudaStream_t stream) {
-  if (wm == 1) launch<D, 1, F16>(p, maps, ctas, device, stream);
-  else if (wm == 2) launch<D, 2, F16>(p, maps, ctas, device, stream);
-  else launch<D, 4, F16>(p, maps, ctas, device, stream);
+  if constexpr (D == 64)
+    if (wm == 2) return launch<D, 2, F16>(p, maps, ctas, device, stream);
+  launch<D, 1, F16>(p, maps, ctas, device, stream);
 }
 
 CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int tok, int heads) {
@@ -603,15 +596,19 @@ CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int to
 }
 
 // The kernel of a call, from the most rows that a unit can have: mma.sync on 16 wm rows, or
-// tcgen05 on nt tiles of 128.
+// tcgen05 on nt tiles of 128.  From 17 rows on tcgen05 wins although it pads them: 32 query heads
+// over 8 KV heads of 128, 16 sequences of 1 to 4 thousand positions, mma.sync against tcgen05: 16
+// rows 38.8 us : 39.3, 32 rows 44.6 : 39.8, 48 rows 54.5 : 41.0, 64 rows 56.4 : 42.5 (mma.sync's
+// warps are bound by the latency of ldmatrix and mma chains, two per scheduler).  At head_dim 64 a
+// block has half the work: 28 rows 14.6 : 17.1, 56 rows 17.6 : 17.2.
 struct Plan {
   int wm, nt, rows, ctas, tile_tok, tpt;
 };
-static Plan plan_of(int group, int max_q, int device) {
+static Plan plan_of(int group, int max_q, int D, int device) {
   const long rows = long(max_q) * group;
   Plan r{};
-  if (rows <= 64) {
-    r.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  if (rows <= (D == 64 ? 32 : 16)) {
+    r.wm = rows <= 16 ? 1 : 2;
     r.rows = 16 * r.wm;
     r.ctas = 2 * sm_count(device);
     r.tpt = r.tile_tok = r.rows / group;
@@ -638,7 +635,7 @@ size_t attention_paged_workspace(const krb_kv_cache &c, int HQ, int max_q) {
   const int group = paged::group_of(c, HQ, max_q);
   int device = 0;
   KRB_CUDA(cudaGetDevice(&device));
-  const paged::Plan pl = paged::plan_of(group, max_q, device);
+  const paged::Plan pl = paged::plan_of(group, max_q, c.head_dim, device);
   return paged::workspace_bytes(pl.ctas, pl.rows, c.head_dim);
 }
 
@@ -665,7 +662,7 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
     throw CudaError("attention_paged: mask rows narrower than max_q");
   int device = 0;
   KRB_CUDA(cudaGetDevice(&device));
-  const Plan pl = plan_of(group, a.max_q, device);
+  const Plan pl = plan_of(group, a.max_q, c.head_dim, device);
   if (!a.workspace || a.workspace_bytes < workspace_bytes(pl.ctas, pl.rows, c.head_dim))
     throw CudaError("attention_paged: workspace too small");
 
@@ -707,8 +704,8 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
     else if (p.D == 128) launch_wm<128, false>(pl.wm, p, maps, pl.ctas, device, stream);
     else if (f16) launch_wm<64, true>(pl.wm, p, maps, pl.ctas, device, stream);
     else launch_wm<64, false>(pl.wm, p, maps, pl.ctas, device, stream);
+    launch_combine(p, pl.ctas, f16, stream);
   }
-  launch_combine(p, pl.ctas, f16, stream);
 }
 
 }  // namespace krb

@@ -27,7 +27,7 @@ struct Params {
   int N, HQ, HKV, group, D;
   int B, max_q, max_pages, pages, page_shift, mask_words;
   int tpt;       // tokens of a unit
-  int tile_tok;  // tokens of one tensor-core tile of the unit (tc kernel; tpt = 1 or 2 tiles)
+  int tile_tok;  // tokens of one 128-row tile of the unit (tcgen05; tpt is one or two tiles)
   int rows;      // rows of a partial result's slot
   float scale_log2;
   uint32_t *status;
@@ -282,13 +282,6 @@ __device__ __forceinline__ float *slot_o(const Params &p, int cta, int slot) {
   return p.o + (static_cast<long>(cta) * 2 + slot) * p.rows * p.D;
 }
 
-// Row of a slot that holds packed row r (token-major: token r / group, head r % group) of a
-// unit: the tc kernel keeps each tile's tokens in 128 rows of its own.
-__device__ __forceinline__ int slot_row(const Params &p, int tok, int g) {
-  const int tile = tok / p.tile_tok;
-  return tile * 128 + (tok - tile * p.tile_tok) * p.group + g;
-}
-
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -308,6 +301,8 @@ struct KvMaps {
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys);
 // q [tokens, HQ, D] with token pitch ldq: boxes of tok x heads x 64
 CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int tok, int heads);
+// a kernel of 128-thread CTAs that is set up while the launch before it drains (it waits by pdl_wait)
+void launch_dependent(void (*kern)(const Params), dim3 grid, const Params &p, cudaStream_t stream);
 // attention_paged_tc.cu
 void launch_tc(const krb_kv_cache &c, int layer, const Params &p, int ctas, int device,
                cudaStream_t stream);

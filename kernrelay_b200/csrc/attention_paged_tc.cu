@@ -6,9 +6,19 @@
 // shared memory), the tile's 128 softmax threads (thread = row) turn S into P in place, and
 // O += P V (P from TMEM, V from shared memory as it lies in the cache, [key][d], so MN-major: no
 // transposed copy).  One warp issues all QK, another all PV, and a tile has two S / P stages in
-// TMEM: scores are a block ahead of the softmax, which never waits for the tensor pipe.
+// TMEM: scores are a block ahead of the softmax.
 //
-// MEASURED
+// Bound: with R rows the products take 4 R 128 D flop per 128 keys for 512 D bytes of K and V, so to
+// about 128 rows HBM binds, beyond it the chip.  Per 128 keys of two tiles the tensor pipe has 2600
+// clocks of work (QK at N = 64 reads 6 KB of shared memory per 32 clocks of products, 128 bytes a
+// clock are there), MUFU 2100; measured are 4000, since a wait on an mbarrier keeps an issuer from
+// feeding the pipe for some 115 clocks even when it has come (its queue holds one or two products).
+// Measured: 64-token trees (8 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads
+// of 128) 63 us, 0.32 of their flop at the library's rate; two chunks of 1024 tokens over 1 and
+// 8 thousand positions 185 us, 0.45; 8-token trees (32 rows, 169 MB) 40 us, 0.65 of the copy's rate.
+// Tried, the trees' and the chunks' time: 128-key blocks with one S stage (70, 205; the chain softmax
+// -> PV -> QK), these with half blocks of P (69, 201) and an issuer per tile (79, 215); one issuer for
+// all products on two stages (83, 239); QK issuers per tile on two stages (69, 203).
 //
 #include <algorithm>
 #include <string>
@@ -125,9 +135,9 @@ __device__ __forceinline__ float exp_block(const uint32_t (&r)[2][32], float sca
 
 // A block of one row: S (64 columns at s_col) -> P over its first 32 columns.  `see`(c): which of
 // the 32 keys of half c the row sees.  P = 2^(s * scale - m) with the row's offset m, which moves
-// only by more than kRescaleLog2; O and l follow it.  The exponentials do not wait for the maximum:
-// they are taken with the old m, and once more where it moves (the first keys of a row, and
-// rarely after).  A row that has seen nothing yet has m = -inf and takes the offset 0.  `o_ready`
+// only by more than kRescaleLog2; O and l follow it.  Behind a piece's first block (`has_o`) the
+// exponentials do not wait for the maximum: they are taken with the old m, and once more where it
+// moves, which is rare.  A row that has seen nothing yet has m = -inf and takes the offset 0.  `o_ready`
 // waits until no product writes O.
 template <int D, bool F16, bool kMask, typename See, typename Ready>
 __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, float scale_log2,
@@ -147,7 +157,8 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
     }
   }
   uint32_t pk[32];
-  float sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
+  float sum = 0.f;
+  if (has_o) sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
   float m8[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) m8[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
@@ -157,7 +168,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
   const float top = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
                           fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * scale_log2;
   const bool grow = top - m_run > kRescaleLog2;
-  if (__any_sync(0xffffffffu, grow)) {
+  if (!has_o || __any_sync(0xffffffffu, grow)) {
     const float alpha = grow ? exp2_mufu(m_run - top) : 1.f;
     if (grow) m_run = top;
     sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
@@ -476,30 +487,42 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
           if (whole) {
             const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
             uint16_t *out = p.out + (w.q0 + t) * p.ldo + static_cast<long>(w.h * p.group + rg) * D;
-#pragma unroll 1
+            uint32_t r[2][32], v[16];
+            tmem_ld_32x32(o_col, r[0]);
+#pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32], v[16];
-              tmem_ld_32x32(o_col + c * 32, r);
               tmem_wait_ld();
+              if (c + 1 < D / 32) tmem_ld_32x32(o_col + (c + 1) * 32, r[(c + 1) & 1]);
 #pragma unroll
               for (int q = 0; q < 16; ++q)
-                v[q] = pack2<F16>(__uint_as_float(r[2 * q]) * inv, __uint_as_float(r[2 * q + 1]) * inv);
+                v[q] = pack2<F16>(__uint_as_float(r[c & 1][2 * q]) * inv,
+                                  __uint_as_float(r[c & 1][2 * q + 1]) * inv);
               store_rows(row_ok ? reinterpret_cast<uint8_t *>(out + c * 32) : nullptr, v);
             }
           } else {
+            // O of a piece lies in 16-byte columns [D / 4][rows][4]: a warp's 32 rows side by side
+            // (row by row, each store touched 32 lines and a piece's end took 8000 clocks)
             const int slot = w.blk == 0, sr = x * 128 + row;
-            float *po = slot_o(p, blockIdx.x, slot) + static_cast<long>(sr) * D;
+            float4 *po = reinterpret_cast<float4 *>(slot_o(p, blockIdx.x, slot)) + sr;
             if (row_ok) {
               float *ml = slot_ml(p, blockIdx.x, slot);
               ml[sr] = m_run;
               ml[p.rows + sr] = l_run;
             }
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t v[16];
-              tmem_ld16(o_col + c * 16, v);
+            uint32_t r[2][32];
+            tmem_ld_32x32(o_col, r[0]);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
               tmem_wait_ld();
-              store_rows(row_ok ? reinterpret_cast<uint8_t *>(po + c * 16) : nullptr, v);
+              if (c + 1 < D / 32) tmem_ld_32x32(o_col + (c + 1) * 32, r[(c + 1) & 1]);
+              const uint32_t(&v)[32] = r[c & 1];
+              if (row_ok) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                  po[(c * 8 + q) * p.rows] =
+                      make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
+                                  __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
+              }
             }
           }
         }
@@ -519,6 +542,75 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ------------------------------------------------------------------ joining split units
+// CTA (c, y, z) joins slot rows 32 y .. and columns z D / 4 .. of the unit that CTA c of the attention
+// kernel began and later ones went on with: a lane per row, a warp per D / 16 columns,
+// O = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) combine_tc_kernel(const Params p) {
+  constexpr int kCols = D / 64;  // 16-byte columns of a lane
+  constexpr int kAhead = 4;      // pieces loaded at a time
+  pdl_wait();
+  const int c = blockIdx.x;
+  const int4 d = p.desc[c];
+  if (d.w < 2) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sr = blockIdx.y * 32 + lane, col = (blockIdx.z * 4 + warp) * kCols;
+  const int tile = sr >> 7, rt = (sr & 127) / p.group, rg = (sr & 127) - rt * p.group;
+  const int tok = tile * p.tile_tok + rt;
+  if (rt >= p.tile_tok || tok >= d.y) return;
+  // running maximum over the groups of pieces
+  float mx = -INFINITY, total = 0.f;
+  float4 acc[kCols];
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < d.w; k0 += kAhead) {
+    float m[kAhead], l[kAhead];
+    float4 v[kAhead][kCols];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int k = k0 + u;
+      m[u] = -INFINITY;
+      if (k >= d.w) continue;
+      const float *ml = slot_ml(p, c + k, k == 0);
+      m[u] = ml[sr];
+      l[u] = ml[p.rows + sr];
+      const float4 *o = reinterpret_cast<const float4 *>(slot_o(p, c + k, k == 0)) + sr;
+#pragma unroll
+      for (int q = 0; q < kCols; ++q) v[u][q] = o[(col + q) * p.rows];
+    }
+    float top = mx;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) top = fmaxf(top, m[u]);
+    const float off = top == -INFINITY ? 0.f : top;
+    const float keep = exp2_mufu(mx - off);
+    mx = top;
+    total *= keep;
+#pragma unroll
+    for (int q = 0; q < kCols; ++q)
+      acc[q] = make_float4(acc[q].x * keep, acc[q].y * keep, acc[q].z * keep, acc[q].w * keep);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (k0 + u >= d.w) continue;
+      const float f = exp2_mufu(m[u] - off);
+      total += f * l[u];
+#pragma unroll
+      for (int q = 0; q < kCols; ++q) {
+        acc[q].x += f * v[u][q].x;
+        acc[q].y += f * v[u][q].y;
+        acc[q].z += f * v[u][q].z;
+        acc[q].w += f * v[u][q].w;
+      }
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  uint16_t *out = p.out + (d.x + tok) * p.ldo + static_cast<long>(d.z * p.group + rg) * D + col * 4;
+#pragma unroll
+  for (int q = 0; q < kCols; ++q)
+    *reinterpret_cast<uint2 *>(out + q * 4) = make_uint2(pack2<F16>(acc[q].x * inv, acc[q].y * inv),
+                                                         pack2<F16>(acc[q].z * inv, acc[q].w * inv));
 }
 
 // ------------------------------------------------------------------ host side
@@ -554,6 +646,9 @@ void launch_tc(const krb_kv_cache &c, int layer, const Params &p, int ctas, int 
   else if (p.D == 128) launch_nt<128, false>(p, tm_q, maps, ctas, device, stream);
   else if (f16) launch_nt<64, true>(p, tm_q, maps, ctas, device, stream);
   else launch_nt<64, false>(p, tm_q, maps, ctas, device, stream);
+  auto *kern = p.D == 128 ? (f16 ? combine_tc_kernel<128, true> : combine_tc_kernel<128, false>)
+                          : (f16 ? combine_tc_kernel<64, true> : combine_tc_kernel<64, false>);
+  launch_dependent(kern, dim3(ctas, p.rows / 32, 4), p, stream);
 }
 
 }  // namespace paged
