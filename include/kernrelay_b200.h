@@ -112,8 +112,8 @@ int krb_attention_prefill_bf16(const void *qkv, void *out, int S, int HQ, int HK
  * Operators of the steps after the prompt; no reference counterpart (the reference runs one
  * prefill).  A cache is two arrays K and V [layers, pages, heads, page_size, head_dim] of
  * 2-byte elements in device memory of the caller, any order of the outer axes: strides in
- * elements of (layer, page, head, slot), head_dim contiguous; k, v 16-byte aligned, strides
- * multiples of 8 whose rows do not overlap.  page_size is a power of two from 8 on, head_dim 64
+ * elements of (layer, page, head, slot), head_dim contiguous; k, v 16-byte aligned and different,
+ * strides multiples of 8 whose rows do not overlap.  page_size is a power of two from 8 on, head_dim 64
  * or 128.  A sequence's tokens live in the pages of its row of a page table (int32 [B,
  * max_pages], row pitch ldp): position p in page table[p / page_size], slot p % page_size.
  * Entries behind a sequence's last page are never read.  max_pages * page_size <= 2^30.

@@ -350,7 +350,8 @@ class KVCache:
 
 def _is(t, dtype, index, dim):
     """A dim-d tensor of dtype on CUDA device `index` whose last axis is contiguous.  These
-    operators' smallest calls take a few microseconds, so their checks are kept as cheap."""
+    operators' smallest calls take a few microseconds, so their checks are kept as cheap (row
+    pitches below: rows that are never stepped over may have any stride)."""
     return (t.dtype is dtype and t.get_device() == index and t.dim() == dim
             and (t.stride(-1) == 1 or t.size(-1) <= 1))
 
@@ -361,18 +362,12 @@ def _refuse(what, name, t, dtype, dim):
                    f"{tuple(t.stride())}")
 
 
-def _pitch(t):
-    """Row pitch of a 2-d tensor (rows that are never stepped over may have any stride)."""
-    rows, width = t.shape
-    return t.stride(0) if rows > 1 else width
-
-
 def _enter(cache):
     """None where the cache's device is the current one, else the context to call again in."""
     import torch
     if cache.index < 0:
         raise KrbError("KVCache: the cache is not on a GPU")
-    if torch.cuda.current_device() == cache.index:
+    if torch._C._cuda_getDevice() == cache.index:  # a CUDA tensor exists: CUDA is initialised
         return None
     return torch.cuda.device(cache.index)
 
@@ -399,15 +394,15 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
     N, width = qkv.shape
     if width != (HQ + 2 * cache.heads) * D:
         raise KrbError(f"{what}: qkv rows must hold (HQ + 2*HKV) * head_dim values")
-    if len(positions) != N or len(slots) != N:
+    if positions.shape[0] != N or slots.shape[0] != N:
         raise KrbError(f"{what}: positions and slots must have one entry per row of qkv")
-    max_pos = len(cos)
-    if (cos.shape != (max_pos, D) or sin.shape != (max_pos, D) or not cos.is_contiguous()
-            or not sin.is_contiguous()):
+    max_pos, columns = cos.shape
+    if columns != D or sin.shape != cos.shape or (max_pos > 1 and (cos.stride(0) != D or sin.stride(0) != D)):
         raise KrbError(f"{what}: cos and sin must be contiguous [max_pos, head_dim]")
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None and not (_is(t, bf, index, 1) and len(t) == D):
-            _refuse(what, f"{name} [head_dim]", t, bf, 1)
+    if q_norm is not None and not (_is(q_norm, bf, index, 1) and q_norm.shape[0] == D):
+        _refuse(what, "q_norm [head_dim]", q_norm, bf, 1)
+    if k_norm is not None and not (_is(k_norm, bf, index, 1) and k_norm.shape[0] == D):
+        _refuse(what, "k_norm [head_dim]", k_norm, bf, 1)
     if status is not None and not _is(status, torch.int32, index, 1):
         _refuse(what, "status", status, torch.int32, 1)
     if out is not None and not (_is(out, dt, index, 2) and out.shape == (N, HQ * D)):
@@ -418,8 +413,10 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
                                       eps, layer, out, status, stream)
     if out is None:
         out = _empty((N, HQ * D), dt, qkv, stream)
+    many = N > 1
     check(lib().krb_qk_norm_rope_paged(
-        cache.ref, layer, qkv.data_ptr(), _pitch(qkv), out.data_ptr(), _pitch(out),
+        cache.ref, layer, qkv.data_ptr(), qkv.stride(0) if many else width, out.data_ptr(),
+        out.stride(0) if many else HQ * D,
         positions.data_ptr(), slots.data_ptr(), N, HQ, cos.data_ptr(), sin.data_ptr(), max_pos,
         _addr(q_norm), _addr(k_norm), eps, _addr(status), _raw_stream(stream, index)), what)
     return out
@@ -449,7 +446,7 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
     if HQ * cache.head_dim != width:
         raise KrbError(f"{what}: q rows must hold HQ * head_dim values")
     B, max_pages = page_table.shape
-    if len(kv_lens) != B or len(q_starts) != B + 1:
+    if kv_lens.shape[0] != B or q_starts.shape[0] != B + 1:
         raise KrbError(f"{what}: page_table, kv_lens and q_starts must be of the same batch")
     words = ldm = 0
     if mask is not None:
@@ -458,7 +455,7 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
         rows, words = mask.shape
         if rows != N:
             raise KrbError(f"{what}: mask must have one row per row of q")
-        ldm = _pitch(mask)
+        ldm = mask.stride(0) if N > 1 else words
     if status is not None and not _is(status, i32, index, 1):
         _refuse(what, "status", status, i32, 1)
     if out is not None and not (_is(out, dt, index, 2) and out.shape == q.shape):
@@ -470,15 +467,17 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
             return attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask,
                                    layer, out, workspace, status, stream)
     need = cache.attention_workspace(HQ, max_q)
+    many = N > 1
     if out is None:
-        out = _empty((N, width), dt, q, stream)
+        out = torch.empty_like(q) if stream is None else _empty((N, width), dt, q, stream)
     if workspace is None:
         workspace = _empty((need,), torch.uint8, q, stream)
     check(lib().krb_attention_paged(
-        cache.ref, layer, q.data_ptr(), _pitch(q), out.data_ptr(), _pitch(out), N, HQ,
-        page_table.data_ptr(), _pitch(page_table), max_pages, kv_lens.data_ptr(),
+        cache.ref, layer, q.data_ptr(), q.stride(0) if many else width, out.data_ptr(),
+        out.stride(0) if many else width, N, HQ, page_table.data_ptr(),
+        page_table.stride(0) if B > 1 else max_pages, max_pages, kv_lens.data_ptr(),
         q_starts.data_ptr(), B, max_q, _addr(mask), ldm, words, scale, workspace.data_ptr(),
-        len(workspace), _addr(status), _raw_stream(stream, index)), what)
+        workspace.shape[0], _addr(status), _raw_stream(stream, index)), what)
     return out
 
 
@@ -518,7 +517,7 @@ def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=No
         _refuse(what, "counts", counts, i32, 1)
     B, A = accepted.shape
     rows, max_pages = page_table.shape
-    if rows != B or len(bases) != B or len(counts) != B:
+    if rows != B or bases.shape[0] != B or counts.shape[0] != B:
         raise KrbError(f"{what}: page_table, bases, accepted and counts must be of the same batch")
     if status is not None and not _is(status, i32, index, 1):
         _refuse(what, "status", status, i32, 1)
@@ -526,8 +525,8 @@ def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=No
         with on:
             return kv_commit(cache, page_table, bases, accepted, counts, status, stream)
     check(lib().krb_kv_commit(
-        cache.ref, page_table.data_ptr(), _pitch(page_table), max_pages, bases.data_ptr(),
-        accepted.data_ptr(), _pitch(accepted), A, counts.data_ptr(), B, _addr(status),
+        cache.ref, page_table.data_ptr(), page_table.stride(0) if B > 1 else max_pages, max_pages,
+        bases.data_ptr(), accepted.data_ptr(), accepted.stride(0) if B > 1 else A, A, counts.data_ptr(), B, _addr(status),
         _raw_stream(stream, index)), what)
 
 

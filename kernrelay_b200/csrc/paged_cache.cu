@@ -12,33 +12,37 @@
 namespace krb {
 
 // ------------------------------------------------------------------ arguments
-static void check_strides(const int64_t *st, const krb_kv_cache &c, const std::string &what) {
+[[noreturn]] static void refuse(const char *what, const char *why) {
+  throw CudaError(std::string(what) + ": " + why);
+}
+
+static void check_strides(const int64_t *st, const krb_kv_cache &c, const char *what) {
   const int64_t n[4] = {c.layers, c.pages, c.heads, c.page_size};
   int order[4] = {0, 1, 2, 3};
   std::sort(order, order + 4, [&](int a, int b) { return st[a] < st[b]; });
   int64_t span = c.head_dim;  // extent of the axes with smaller strides, in elements
   for (int i : order) {
     if (n[i] == 1) continue;  // never stepped along
-    if (st[i] % 8) throw CudaError(what + ": cache strides must be multiples of 8 elements");
-    if (st[i] < span) throw CudaError(what + ": cache strides overlap");
-    if (st[i] > (int64_t(1) << 38)) throw CudaError(what + ": cache stride too large");
+    if (st[i] % 8) refuse(what, "cache strides must be multiples of 8 elements");
+    if (st[i] < span) refuse(what, "cache strides overlap");
+    if (st[i] > (int64_t(1) << 38)) refuse(what, "cache stride too large");
     span = st[i] * (n[i] - 1) + span;
   }
 }
 
-void check_cache(const krb_kv_cache *c, int layer, const char *name) {
-  const std::string what(name);
-  if (!c) throw CudaError(what + ": no cache");
-  if (!c->k || !c->v) throw CudaError(what + ": cache without K or V");
+void check_cache(const krb_kv_cache *c, int layer, const char *what) {
+  if (!c) refuse(what, "no cache");
+  if (!c->k || !c->v) refuse(what, "cache without K or V");
+  if (c->k == c->v) refuse(what, "K and V are the same array");
   if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
-    throw CudaError(what + ": K and V must be 16-byte aligned");
-  if (c->dtype != 0 && c->dtype != 1) throw CudaError(what + ": cache dtype must be bf16 or fp16");
+    refuse(what, "K and V must be 16-byte aligned");
+  if (c->dtype != 0 && c->dtype != 1) refuse(what, "cache dtype must be bf16 or fp16");
   if (c->layers <= 0 || c->pages <= 0 || c->heads <= 0)
-    throw CudaError(what + ": cache without layers, pages or heads");
-  if (c->head_dim != 64 && c->head_dim != 128) throw CudaError(what + ": head_dim must be 64 or 128");
+    refuse(what, "cache without layers, pages or heads");
+  if (c->head_dim != 64 && c->head_dim != 128) refuse(what, "head_dim must be 64 or 128");
   if (c->page_size < 8 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)))
-    throw CudaError(what + ": page_size must be a power of two from 8 on");
-  if (layer < 0 || layer >= c->layers) throw CudaError(what + ": no such layer");
+    refuse(what, "page_size must be a power of two from 8 on");
+  if (layer < 0 || layer >= c->layers) refuse(what, "no such layer");
   check_strides(c->k_stride, *c, what);
   check_strides(c->v_stride, *c, what);
 }
@@ -385,17 +389,19 @@ void kv_copy_pages(const krb_kv_cache &c, const int32_t *src, const int32_t *dst
   if (n < 0) throw CudaError("kv_copy_pages: negative count");
   if (n == 0) return;
   if (!src || !dst) throw CudaError("kv_copy_pages: null pointer");
-  std::vector<char> written(c.pages, 0);
+  std::vector<int32_t> written;  // in order
+  written.reserve(n);
   for (int i = 0; i < n; ++i) {
     for (const int32_t p : {src[i], dst[i]})
       if (p < 0 || p >= c.pages) throw CudaError("kv_copy_pages: no page " + std::to_string(p));
-    if (src[i] == dst[i]) continue;
-    if (written[dst[i]])
-      throw CudaError("kv_copy_pages: page " + std::to_string(dst[i]) + " is written twice");
-    written[dst[i]] = 1;
+    if (src[i] != dst[i]) written.push_back(dst[i]);
   }
+  std::sort(written.begin(), written.end());
+  const auto twice = std::adjacent_find(written.begin(), written.end());
+  if (twice != written.end())
+    throw CudaError("kv_copy_pages: page " + std::to_string(*twice) + " is written twice");
   for (int i = 0; i < n; ++i)
-    if (src[i] != dst[i] && written[src[i]])
+    if (src[i] != dst[i] && std::binary_search(written.begin(), written.end(), src[i]))
       throw CudaError("kv_copy_pages: page " + std::to_string(src[i]) + " is read and written");
   CopyArgs a;
   const int64_t *strides[2] = {c.k_stride, c.v_stride};

@@ -20,6 +20,7 @@ def _message(krlib):
 
 BAD_CACHES = [
     (dict(k=0), "without K or V"), (dict(v=0), "without K or V"), (dict(k=4104), "aligned"),
+    (dict(v=4096), "same array"),
     (dict(dtype=2), "dtype"), (dict(layers=0), "layers"), (dict(pages=-1), "pages"),
     (dict(heads=0), "heads"), (dict(head_dim=96), "head_dim"), (dict(page_size=24), "power of two"),
     (dict(page_size=4), "power of two"),
