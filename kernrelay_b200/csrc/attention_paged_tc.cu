@@ -117,20 +117,52 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr) {
 __device__ __forceinline__ int k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int v_at(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * j + 1; }
 
+// two fp32 values in a register pair: one instruction for both
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // P = 2^(s * scale - off) of 64 scores, packed in the cache's type, and their sum in fp32.
 template <bool F16>
-__device__ __forceinline__ float exp_block(const uint32_t (&r)[2][32], float scale_log2, float off,
-                                          uint32_t (&pk)[32]) {
-  float r8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ float exp_block(const uint32_t (&s)[2][32], float scale_log2, float off,
+                                           uint32_t (&pk)[32]) {
+  const uint64_t sc = pack_f32x2(__float_as_uint(scale_log2), __float_as_uint(scale_log2));
+  const uint64_t mo = pack_f32x2(__float_as_uint(-off), __float_as_uint(-off));
+  uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < 32; ++e) {
-    const float p0 = exp2_mufu(fmaf(__uint_as_float(r[e >> 4][(2 * e) & 31]), scale_log2, -off));
-    const float p1 = exp2_mufu(fmaf(__uint_as_float(r[e >> 4][(2 * e + 1) & 31]), scale_log2, -off));
+    const uint64_t x = pack_f32x2(s[e >> 4][(2 * e) & 31], s[e >> 4][(2 * e + 1) & 31]);
+    const float2 a = unpack_f32x2(fma_f32x2(x, sc, mo));
+    const float p0 = exp2_mufu(a.x), p1 = exp2_mufu(a.y);
     // P in the cache's type (its rounding is that of the output); the row sum takes the fp32 values
+    // (the rounded ones gave the same error for a tenth more time)
     pk[e] = pack2<F16>(p0, p1);
-    r8[e & 7] += p0 + p1;
+    sum[e & 3] = add_f32x2(sum[e & 3], pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
   }
-  return ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
+  const float2 t = unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
+  return t.x + t.y;
 }
 
 // A block of one row: S (64 columns at s_col) -> P over its first 32 columns.  `see`(c): which of
@@ -159,14 +191,13 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
   uint32_t pk[32];
   float sum = 0.f;
   if (has_o) sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
-  float m8[8];
+  float m4[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m8[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
+  for (int e = 0; e < 4; ++e) m4[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
 #pragma unroll
-  for (int e = 8; e < 32; ++e)
-    m8[e & 7] = fmaxf(m8[e & 7], fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e])));
-  const float top = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                          fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * scale_log2;
+  for (int e = 4; e < 32; ++e)
+    m4[e & 3] = max3(m4[e & 3], __uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
+  const float top = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * scale_log2;
   const bool grow = top - m_run > kRescaleLog2;
   if (!has_o || __any_sync(0xffffffffu, grow)) {
     const float alpha = grow ? exp2_mufu(m_run - top) : 1.f;
