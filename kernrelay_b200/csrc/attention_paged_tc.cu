@@ -222,15 +222,12 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
   tmem_wait_st();
 }
 
-// 64 bytes of this thread's row (null: it has none)
+// 64 bytes of this thread's row (null: it has none); rows are 16-byte aligned
 __device__ __forceinline__ void store_rows(uint8_t *dst, const uint32_t (&v)[16]) {
   if (!dst) return;
 #pragma unroll
-  for (int q = 0; q < 16; q += 8)
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 4 * q), "r"(v[q]),
-                 "r"(v[q + 1]), "r"(v[q + 2]), "r"(v[q + 3]), "r"(v[q + 4]), "r"(v[q + 5]), "r"(v[q + 6]),
-                 "r"(v[q + 7])
-                 : "memory");
+  for (int q = 0; q < 4; ++q)
+    reinterpret_cast<uint4 *>(dst)[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
 
 }  // namespace

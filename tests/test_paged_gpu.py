@@ -344,6 +344,34 @@ def test_groups(cuda, krlib, HQ, HKV, D, T):
     b.check(out)
 
 
+@pytest.mark.parametrize("T", [1, 3, 30, 200])
+@pytest.mark.parametrize("HQ,HKV,D", [(28, 4, 128), (14, 2, 64)])
+def test_output_rows_16_byte_aligned(cuda, krlib, T, HQ, HKV, D):
+    """Output rows at every multiple of 16 bytes, whole units and split ones; what lies between
+    them stays."""
+    import torch
+    b = Batch([(300, T), (0, T), (1000, 1)], HQ, HKV, D, 16, "fp16", seed=T)
+    for lead, tail in ((8, 0), (8, 8), (24, 16)):
+        wide = torch.full((b.N, lead + HQ * D + tail + 8), 5.0, dtype=b.dt, device="cuda")
+        out = wide[:, lead:lead + HQ * D]
+        b.run(krlib, out=out)
+        torch.cuda.synchronize()
+        assert b.status.item() == 0
+        b.check(out)
+        assert (wide[:, :lead] == 5.0).all() and (wide[:, lead + HQ * D:] == 5.0).all()
+
+
+@pytest.mark.parametrize("T,HQ,HKV,D", [(200, 14, 2, 64), (130, 4, 4, 128), (300, 8, 1, 128)])
+def test_wide_tree(cuda, krlib, T, HQ, HKV, D):
+    """Masks of many words, over several units of a sequence."""
+    import torch
+    b = Batch([(70, T), (0, T), (500, 3)], HQ, HKV, D, 32, "bf16", masked=True, seed=T, empty={1})
+    out = b.run(krlib)
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    b.check(out)
+
+
 def test_many_sequences(cuda, krlib):
     """More sequences than a warp's lanes, and than CTAs; several without new tokens."""
     import torch
@@ -581,6 +609,27 @@ def test_commit(cuda, krlib, layout, layers, heads, page, D, T, dtype):
     torch.cuda.synchronize()
     assert status.item() == 0
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_commit_long_list(cuda, krlib):
+    """More accepted tokens than a CTA keeps at a time (a prompt's rows closed up)."""
+    import torch
+    g, rng = _gen(9), random.Random(9)
+    page, T, n = 16, 900, 700
+    k, v = _cache_tensors(2, T // page + 2, 2, page, 64, torch.float16, "hnd", g=g)
+    ids = list(range(k.shape[1]))
+    rng.shuffle(ids)
+    acc = sorted(rng.sample(range(T), n))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    want = []
+    for t in (k, v):
+        flat = t[:, ids].transpose(2, 3).reshape(2, -1, 2, 64).clone()  # by position
+        flat[:, 3:3 + n] = flat[:, [3 + a for a in acc]]
+        want.append(flat)
+    krlib.kv_commit(krlib.KVCache(k, v), i32([ids]), i32([3]), i32([acc]), i32([n]))
+    torch.cuda.synchronize()
+    for t, w in zip((k, v), want):
+        assert torch.equal(t[:, ids].transpose(2, 3).reshape(2, -1, 2, 64), w)
 
 
 def test_commit_refuses_per_sequence(cuda, krlib):
