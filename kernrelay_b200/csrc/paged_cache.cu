@@ -260,22 +260,20 @@ constexpr int kCommitList = 256;
 template <int D>
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
   constexpr int kLanes = D / 8;
-  __shared__ int s_bad;
   __shared__ int4 s_move[kCommitList];  // source page, slot; target page, slot (source page -1: stays)
   const int b = blockIdx.x;
-  const int n = a.counts[b];
-  const int64_t base = a.bases[b];
-  const int64_t room = static_cast<int64_t>(a.max_pages) << a.page_shift;
-  const bool sizes_ok = n >= 0 && n <= a.A && base >= 0 && base <= room;
-  if (threadIdx.x == 0) s_bad = !sizes_ok;
-  __syncthreads();
   const int32_t *acc = a.accepted + b * a.lda;
   const int32_t *table = a.page_table + b * a.ldp;
+  const int t = threadIdx.x;
+  // the list's first entries come with the sizes, not behind them
+  const int n = a.counts[b];
+  const int64_t base = a.bases[b];
+  const int first = t < a.A ? acc[t] : 0, before_first = t > 0 && t < a.A ? acc[t - 1] : -1;
+  const int64_t room = static_cast<int64_t>(a.max_pages) << a.page_shift;
+  const bool sizes_ok = n >= 0 && n <= a.A && base >= 0 && base <= room;
   const int slot_mask = (1 << a.page_shift) - 1;
-  // move i of the list, checked
-  auto move = [&](int i, int4 &m) {
-    const int64_t x = acc[i];
-    const int64_t before = i ? acc[i - 1] : -1;
+  // the move of entry i = x, checked
+  auto move = [&](int i, int64_t x, int64_t before, int4 &m) {
     if (x <= before || base + x >= room) return false;
     const int64_t from = base + x, to = base + i;
     m = make_int4(table[from >> a.page_shift], static_cast<int>(from) & slot_mask,
@@ -284,16 +282,16 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
     if (x == i) m.x = -1;
     return true;
   };
+  bool bad = !sizes_ok;
   if (sizes_ok) {
-    for (int i = threadIdx.x; i < n; i += kCommitThreads) {
+    for (int i = t; i < n; i += kCommitThreads) {
       int4 m;
-      if (!move(i, m)) s_bad = 1;
+      if (!move(i, i == t ? first : acc[i], i == t ? before_first : acc[i - 1], m)) bad = true;
       else if (i < kCommitList) s_move[i] = m;
     }
   }
-  __syncthreads();
-  if (s_bad) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) report_status(a.status, kStatusBadIndex);
+  if (__syncthreads_or(bad)) {
+    if (t == 0 && blockIdx.y == 0) report_status(a.status, kStatusBadIndex);
     return;
   }
   const int rows = a.layers * 2 * a.heads;
@@ -308,7 +306,7 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs
     if (l0 > 0) {  // the next part of a long list
       __syncthreads();
       for (int i = l0 + threadIdx.x; i < min(n, l0 + kCommitList); i += kCommitThreads)
-        move(i, s_move[i - l0]);
+        move(i, acc[i], acc[i - 1], s_move[i - l0]);
       __syncthreads();
     }
     if (row >= rows) continue;
