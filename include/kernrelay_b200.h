@@ -155,7 +155,10 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * anything.  max_q bounds every T_b, HQ / HKV <= 64, scale > 0.  T_b = 0 is allowed.
  * A sequence with T_b > max_q, kv_lens[b] < T_b or > max_pages * page_size, or rows outside
  * [0, N) sets bit 7 and its rows are left as they were, like rows that belong to no sequence.
+ * (So does, for the whole call, a sequence of more than 2^26 blocks of 64 keys, its row tiles and
+ * KV heads counted each, or 2^31 in all.)
  * A page outside [0, pages) sets bit 8 and is read as page 0.
+ * out must not overlap q.
  * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call
  * alone until it is done; calls in order on one stream may share one. */
 int krb_attention_paged(const krb_kv_cache *cache, int layer, const void *q, int64_t ldq,

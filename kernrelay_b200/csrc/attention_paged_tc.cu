@@ -13,10 +13,11 @@
 // clocks of work (QK at N = 64 reads 6 KB of shared memory per 32 clocks of products, 128 bytes a
 // clock are there), MUFU 2100; measured are 4000, since a wait on an mbarrier keeps an issuer from
 // feeding the pipe for some 115 clocks even when it has come (its queue holds one or two products).
+// A piece's start and end (first scores, last product, O out) cost some 5000 more.
 // Measured: 64-token trees (8 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads
-// of 128) 63 us, 0.32 of their flop at the library's rate; two chunks of 1024 tokens over 1 and
-// 8 thousand positions 185 us, 0.45; 8-token trees (32 rows, 169 MB) 40 us, 0.65 of the copy's rate.
-// Tried, the trees' and the chunks' time: 128-key blocks with one S stage (70, 205; the chain softmax
+// of 128) 62 us, 0.32 of their flop at the library's rate; two chunks of 1024 tokens over 1 and
+// 8 thousand positions 187 us, 0.44; 8-token trees (32 rows, 169 MB) 40 us, 0.65 of the copy's rate.
+// Tried, the trees' and the chunks' time: 128-key blocks with one S stage (70, 205: the chain softmax
 // -> PV -> QK), these with half blocks of P (69, 201) and an issuer per tile (79, 215); one issuer for
 // all products on two stages (83, 239); QK issuers per tile on two stages (69, 203).
 //
@@ -116,33 +117,6 @@ __device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr) {
 // K0, K1, V0, K2, V1, ... (K of the next block before V of this one).
 __device__ __forceinline__ int k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int v_at(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * j + 1; }
-
-// two fp32 values in a register pair: one instruction for both
-__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 
 // P = 2^(s * scale - off) of 64 scores, packed in the cache's type, and their sum in fp32.
 template <bool F16>

@@ -71,25 +71,30 @@ struct AppendArgs {
   uint32_t *status;
 };
 
+// eight 2-byte values as four pairs of fp32, and back
 template <bool F16>
-__device__ __forceinline__ void unpack8(const uint4 &w, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4 &w, uint64_t (&f)[4]) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float2 t = unpack2<F16>(ws[e]);
-    f[2 * e] = t.x;
-    f[2 * e + 1] = t.y;
+    if constexpr (F16) {
+      const float2 t = unpack2<true>(ws[e]);
+      f[e] = pack_f32x2(__float_as_uint(t.x), __float_as_uint(t.y));
+    } else {
+      f[e] = pack_f32x2(ws[e] << 16, ws[e] & 0xffff0000u);
+    }
   }
 }
 
 template <bool F16>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 w;
-  w.x = pack2<F16>(f[0], f[1]);
-  w.y = pack2<F16>(f[2], f[3]);
-  w.z = pack2<F16>(f[4], f[5]);
-  w.w = pack2<F16>(f[6], f[7]);
-  return w;
+__device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 t = unpack_f32x2(f[e]);
+    w[e] = pack2<F16>(t.x, t.y);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ uint4 ldg4(const void *p) {
@@ -104,10 +109,11 @@ __device__ __forceinline__ uint4 ldg4(const void *p) {
 //
 // Bound: HBM at size (every value read and written once), a launch when small.  What it takes is
 // loads in flight, and that is warps: the halves are rotated one after the other so that five CTAs
-// are resident (4 / 5 / 6 by the register limit: 48.8 / 44.2 / 45.6 us for 8192 tokens of 32 + 2 x 8
-// heads of 128 with norms, 203 MB, 31.6 us at the copy's rate; 8192 tokens of 14 + 2 x 2 heads of 64
-// 8.7 / 8.2 / 9.0).  Tried: several heads per warp with the table products in registers (54 us, 14.5),
-// and whole rows by bulk copies into shared memory (42.2 us, but 17.1).
+// are resident, in paired fp32 (5 / 6 by the register limit: 42.7 / 42.9 us for 8192 tokens of 32 + 2
+// x 8 heads of 128 with norms, 203 MB, 31.6 us at the copy's rate; 8.3 / 8.3 for 8192 tokens of 14 + 2
+// x 2 heads of 64; unpaired 48.8 / 44.2 / 45.6 with 4 / 5 / 6).  Tried: several heads per warp with the
+// table products in registers (54 us, 14.5), and whole rows by bulk copies into shared memory (42.2
+// us, but 17.1).
 template <int D, bool F16>
 __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
@@ -155,37 +161,44 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
   const long t = pos * D + j;
   const uint4 tc0 = ldg4(a.cos_tab + t), ts0 = ldg4(a.sin_tab + t);
   const uint4 tc1 = ldg4(a.cos_tab + t + HALF), ts1 = ldg4(a.sin_tab + t + HALF);
-  float lo[8], hi[8];
+  uint64_t lo[4], hi[4], f[4];
   unpack8<F16>(wlo, lo);
   unpack8<F16>(whi, hi);
   const __nv_bfloat16 *nw = h < a.HQ ? a.q_norm : a.k_norm;
   if (nw) {
-    float ss = 0.f;
+    uint64_t sq = 0;  // two sums
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+    for (int e = 0; e < 4; ++e) sq = fma_f32x2(hi[e], hi[e], fma_f32x2(lo[e], lo[e], sq));
+    const float2 s2 = unpack_f32x2(sq);
+    float ss = s2.x + s2.y;
     const unsigned lane = threadIdx.x & 31;
     const unsigned mask = ((1u << kLanes) - 1u) << (lane & ~unsigned(kLanes - 1));
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-    const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-    float w[8];
-    unpack8<false>(ldg4(nw + j), w);
+    const uint32_t r = __float_as_uint(rsqrtf(ss * (1.0f / D) + a.eps));
+    const uint64_t rr = pack_f32x2(r, r);
+    unpack8<false>(ldg4(nw + j), f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] *= r * w[e];
-    unpack8<false>(ldg4(nw + HALF + j), w);
+    for (int e = 0; e < 4; ++e) lo[e] = mul_f32x2(lo[e], mul_f32x2(rr, f[e]));
+    unpack8<false>(ldg4(nw + HALF + j), f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hi[e] *= r * w[e];
+    for (int e = 0; e < 4; ++e) hi[e] = mul_f32x2(hi[e], mul_f32x2(rr, f[e]));
   }
-  float c[8], s[8], y[8];
-  unpack8<false>(tc0, c);
-  unpack8<false>(ts0, s);
+  uint64_t y[4];
+  unpack8<false>(tc0, f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = lo[e] * c[e] - hi[e] * s[e];
+  for (int e = 0; e < 4; ++e) y[e] = mul_f32x2(lo[e], f[e]);
+  unpack8<false>(make_uint4(ts0.x ^ 0x80008000u, ts0.y ^ 0x80008000u, ts0.z ^ 0x80008000u,
+                            ts0.w ^ 0x80008000u), f);  // -sin
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fma_f32x2(hi[e], f[e], y[e]);
   *reinterpret_cast<uint4 *>(dst) = pack8<F16>(y);
-  unpack8<false>(tc1, c);
-  unpack8<false>(ts1, s);
+  unpack8<false>(tc1, f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = hi[e] * c[e] + lo[e] * s[e];
+  for (int e = 0; e < 4; ++e) y[e] = mul_f32x2(hi[e], f[e]);
+  unpack8<false>(ts1, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fma_f32x2(lo[e], f[e], y[e]);
   *reinterpret_cast<uint4 *>(dst + HALF) = pack8<F16>(y);
 }
 
