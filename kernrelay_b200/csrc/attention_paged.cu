@@ -93,7 +93,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -103,6 +102,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     fence_mbar_init();
   }
+  pdl_wait();
+  pdl_launch_dependents();
   if (warp < 4) prefetch_page_table(p, threadIdx.x, kConsumers);
   if (warp == 4) {
     const Walk s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
@@ -515,23 +516,10 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ host side
-void launch_dependent(void (*kern)(const Params), dim3 grid, const Params &p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  KRB_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
-}
-
 static void launch_combine(const Params &p, int ctas, bool f16, cudaStream_t stream) {
   auto *kern = p.D == 128 ? (f16 ? combine_kernel<128, true> : combine_kernel<128, false>)
                           : (f16 ? combine_kernel<64, true> : combine_kernel<64, false>);
-  launch_dependent(kern, dim3(ctas, std::min(p.tpt, p.max_q) * p.group), p, stream);
+  launch_pdl(kern, dim3(ctas, std::min(p.tpt, p.max_q) * p.group), 128, 0, stream, true, p);
 }
 
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys) {
@@ -577,8 +565,7 @@ static void launch(const Params &p, const KvMaps &maps, int ctas, int device, cu
   }
   int box_shift = 0;
   while ((1 << box_shift) < maps.box) ++box_shift;
-  kern<<<ctas, kThreads, Cfg<D>::kSmem, stream>>>(maps.k, maps.v, p, box_shift);
-  KRB_CUDA(cudaGetLastError());
+  launch_pdl(kern, dim3(ctas), kThreads, Cfg<D>::kSmem, stream, false, maps.k, maps.v, p, box_shift);
 }
 
 template <int D, bool F16>

@@ -282,11 +282,6 @@ __device__ __forceinline__ float *slot_o(const Params &p, int cta, int slot) {
   return p.o + (static_cast<long>(cta) * 2 + slot) * p.rows * p.D;
 }
 
-__device__ __forceinline__ void pdl_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ float exp2_mufu(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -301,8 +296,6 @@ struct KvMaps {
 KvMaps make_kv_maps(const krb_kv_cache &c, int layer, int keys);
 // q [tokens, HQ, D] with token pitch ldq: boxes of tok x heads x 64
 CUtensorMap make_tmap_rows(const void *q, int N, int HQ, int D, long ldq, int tok, int heads);
-// a kernel of 128-thread CTAs that is set up while the launch before it drains (it waits by pdl_wait)
-void launch_dependent(void (*kern)(const Params), dim3 grid, const Params &p, cudaStream_t stream);
 // attention_paged_tc.cu
 void launch_tc(const krb_kv_cache &c, int layer, const Params &p, int ctas, int device,
                cudaStream_t stream);

@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 32) {
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&full[i], 1);
@@ -243,13 +242,15 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
     }
     fence_mbar_init();
   }
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
   if (warp >= 2) prefetch_page_table(p, threadIdx.x - 64, C::kThreads - 64);
   if (warp == 0) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_q);
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-    }
     const Walk s = find_start<kKeys>(p, blockIdx.x, gridDim.x);
     if (lane == 0) *start = s;
   } else if (warp == 1) {
@@ -628,8 +629,7 @@ static void launch(const Params &p, const CUtensorMap &tm_q, const KvMaps &maps,
   }
   int box_shift = 0;
   while ((1 << box_shift) < maps.box) ++box_shift;
-  kern<<<ctas, C::kThreads, C::kSmem, stream>>>(tm_q, maps.k, maps.v, p, box_shift);
-  KRB_CUDA(cudaGetLastError());
+  launch_pdl(kern, dim3(ctas), C::kThreads, C::kSmem, stream, false, tm_q, maps.k, maps.v, p, box_shift);
 }
 
 template <int D, bool F16>
@@ -650,7 +650,7 @@ void launch_tc(const krb_kv_cache &c, int layer, const Params &p, int ctas, int 
   else launch_nt<64, false>(p, tm_q, maps, ctas, device, stream);
   auto *kern = p.D == 128 ? (f16 ? combine_tc_kernel<128, true> : combine_tc_kernel<128, false>)
                           : (f16 ? combine_tc_kernel<64, true> : combine_tc_kernel<64, false>);
-  launch_dependent(kern, dim3(ctas, p.rows / 32, 4), p, stream);
+  launch_pdl(kern, dim3(ctas, p.rows / 32, 4), 128, 0, stream, true, p);
 }
 
 }  // namespace paged

@@ -1,10 +1,34 @@
 // The paged K/V cache as the kernels see it, and the launchers of its operators.
 #pragma once
 
+#include <utility>
+
 #include "common.h"
 #include "kernrelay_b200.h"
 
 namespace krb {
+
+// Launch by programmatic dependent launch: `kern` waits for the work before it itself (pdl_wait, first
+// thing).  The gap between launches on a stream falls from 2.3 to about 1 us.  `always`: in a
+// capture, too (behind a kernel of the same call); else a captured launch takes plain dependencies,
+// whatever the stream waits for.
+template <typename... P, typename... A>
+void launch_pdl(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, bool always,
+                A &&...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (!always) KRB_CUDA(cudaStreamIsCapturing(stream, &status));
+  cfg.numAttrs = status == cudaStreamCaptureStatusNone ? 1 : 0;
+  KRB_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
+}
 
 // Throws on a cache the operators do not take (null pointers, sizes, alignment, strides whose
 // rows overlap); `layer` in [0, layers).

@@ -118,6 +118,7 @@ template <int D, bool F16>
 __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
   constexpr int kLanes = HALF / 8;
+  pdl_wait();
   const uint32_t gt = blockIdx.x * 256u + threadIdx.x;
   const uint32_t nh = a.HQ + 2 * a.HKV;
   const uint32_t item = gt / kLanes;
@@ -206,7 +207,7 @@ template <int D, bool F16>
 void launch_append(const AppendArgs &a, cudaStream_t stream) {
   const long threads = static_cast<long>(a.N) * (a.HQ + 2 * a.HKV) * (D / 16);
   if (threads > 0xffffff00L) throw CudaError("qk_norm_rope_paged: too many tokens");
-  append_kernel<D, F16><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(a);
+  launch_pdl(append_kernel<D, F16>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0, stream, false, a);
 }
 
 // ------------------------------------------------------------------ page copies
@@ -229,6 +230,7 @@ constexpr int kCopyVec = 4;
 
 // grid (chunks of a page, pairs, layers * 2): 256 threads move kCopyVec units each
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+  pdl_wait();
   const int kv = blockIdx.z & 1;
   const int layer = blockIdx.z >> 1;
   const long base = layer * a.layer[kv];
@@ -274,6 +276,7 @@ template <int D>
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
   constexpr int kLanes = D / 8;
   __shared__ int4 s_move[kCommitList];  // source page, slot; target page, slot (source page -1: stays)
+  pdl_wait();
   const int b = blockIdx.x;
   const int32_t *acc = a.accepted + b * a.lda;
   const int32_t *table = a.page_table + b * a.ldp;
@@ -392,7 +395,6 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
   else if (D == 128) launch_append<128, false>(a, stream);
   else if (c.dtype) launch_append<64, true>(a, stream);
   else launch_append<64, false>(a, stream);
-  KRB_CUDA(cudaGetLastError());
 }
 
 void kv_copy_pages(const krb_kv_cache &c, const int32_t *src, const int32_t *dst, int n,
@@ -458,8 +460,7 @@ void kv_copy_pages(const krb_kv_cache &c, const int32_t *src, const int32_t *dst
     }
     if (!m) break;
     const dim3 grid((a.units + 256 * kCopyVec - 1) / (256 * kCopyVec), m, 2 * c.layers);
-    copy_pages_kernel<<<grid, 256, 0, stream>>>(a);
-    KRB_CUDA(cudaGetLastError());
+    launch_pdl(copy_pages_kernel, grid, 256, 0, stream, false, a);
   }
 }
 
@@ -502,9 +503,8 @@ void kv_commit(const krb_kv_cache &c, const int32_t *page_table, long ldp, int m
   const long gy = (rows + per - 1) / per;
   if (gy > 65535) throw CudaError("kv_commit: too many layers and heads");
   const dim3 grid(B, static_cast<unsigned>(gy));
-  if (c.head_dim == 128) commit_kernel<128><<<grid, kCommitThreads, 0, stream>>>(a);
-  else commit_kernel<64><<<grid, kCommitThreads, 0, stream>>>(a);
-  KRB_CUDA(cudaGetLastError());
+  launch_pdl(c.head_dim == 128 ? commit_kernel<128> : commit_kernel<64>, grid, kCommitThreads, 0, stream,
+             false, a);
 }
 
 }  // namespace krb

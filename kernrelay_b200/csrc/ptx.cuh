@@ -439,6 +439,15 @@ __device__ __forceinline__ float2 unpack_f16x2(uint32_t u) {
   return __half22float2(v);
 }
 
+// ---------------------------------------------------------------- programmatic dependent launch
+// A kernel launched with it may be set up while the one before it on the stream drains; pdl_wait
+// returns when that one is complete and its writes are visible, so it comes before every access to
+// global memory.
+__device__ __forceinline__ void pdl_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- paired fp32 arithmetic
 // two fp32 values in a register pair: one instruction for both
 __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {

@@ -493,6 +493,55 @@ def test_streams_and_workspace(cuda, krlib):
             assert torch.equal(x, w)
 
 
+@pytest.mark.parametrize("T", [1, 40])
+def test_order_across_streams(cuda, krlib, T):
+    """Each operator starts behind the work before it on its stream, and behind what that stream was
+    told to wait for, although its launch is set up early: producers kept busy on either."""
+    import torch
+    HQ, HKV, D, page, n = 8, 2, 128, 16, 512
+    g, dt = _gen(T), torch.bfloat16
+    k, v = _cache_tensors(1, 2 * n // page + 2, HKV, page, D, dt, "hnd", fill=0.0)
+    cache = krlib.KVCache(k, v)
+    cos, sin = _rope_tables(n + 1, D)
+    table = torch.arange(k.shape[1], dtype=torch.int32, device="cuda")[None]
+    pos = torch.arange(n, device="cuda")
+    lens, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([n], [0, T]))
+    busy = torch.randn(4096, 4096, generator=g, device="cuda")
+    rows = torch.randn(6, n, (HQ + 2 * HKV) * D, generator=g, device="cuda").to(dt)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    src = torch.empty_like(rows[0])
+    scale = 1 / math.sqrt(D)
+
+    def step(x, s1, s2):
+        with torch.cuda.stream(s1):
+            (busy @ busy).sum()
+            src.copy_(x)
+            q = krlib.qk_norm_rope_paged(src, cache, pos, pos, HQ, cos, sin)
+            (busy @ busy).sum()
+            krlib.kv_copy_pages(cache, [0, 1], [n // page + 1, n // page])
+            done = torch.cuda.Event()
+            done.record()
+        with torch.cuda.stream(s2):
+            s2.wait_event(done)
+            out = krlib.attention_paged(q[n - T:], cache, table, lens, starts, T, scale)
+            held = torch.stack([k[0, n // page + 1], k[0, n // page]])
+            back = torch.cuda.Event()
+            back.record()
+        q.record_stream(s2)
+        s1.wait_event(back)
+        return out, held
+
+    torch.cuda.synchronize()
+    want = [step(x, a, a) for x in rows]
+    torch.cuda.synchronize()
+    got = [step(x, a, b) for x in rows]
+    torch.cuda.synchronize()
+    for i, ((o1, h1), (o2, h2)) in enumerate(zip(want, got)):
+        assert torch.equal(o1, o2) and torch.equal(h1, h2), i
+    for (o1, _), (o2, _) in zip(want, want[1:]):
+        assert not torch.equal(o1, o2)
+
+
 def test_graph_follows_lengths(cuda, krlib):
     """A captured call reads lengths and pages when it is replayed."""
     import torch
