@@ -8,7 +8,8 @@ Tolerances (u = half a step of the 2-byte type, eps / 2):
   sum takes them unrounded), and the scores' fp32 error: D + 4 roundings of 2^-24 of
   S = scale * sum_d |q_d k_d| change a probability by twice that, relative; the sums over n keys
   n 2^-24 (of fp32 products, whose order is free), exp2 2^-21.  fp16 probabilities below 2^-14
-  have an absolute error, 2^-25, where the row's largest is at least 1: 2^-25 sum_j |v_j|.
+  have an absolute error, 2^-25, where the row's largest is at least 1: 2^-25 sum_j |v_j|; so does
+  an fp16 output below 2^-14 (its neighbours are 2^-24 apart): 2^-25.
 * copies and commits: the same bits."""
 import math
 import random
@@ -176,7 +177,7 @@ def _tree(rng, t, words, empty=()):
     # bits behind the last token are the caller's: set them
     sees = [x | (((1 << (32 * words - t)) - 1) << t) for x in sees]
     rows = [[(x >> (32 * w)) & 0xFFFFFFFF for w in range(words)] for x in sees]
-    return torch.tensor(rows, dtype=torch.int64).to(torch.int32), seen
+    return torch.tensor(rows, dtype=torch.int64).to(torch.int32).view(t, words), seen.view(t, t)
 
 
 class Batch:
@@ -264,7 +265,7 @@ class Batch:
             rel = 2 * (D + 4) * 2.0 ** -24 * S + n * 2.0 ** -24 + 2.0 ** -20
             bound = u * ref.abs() + (u + rel) * A * (1 + 2 * u)
             if self.dt == torch.float16:
-                bound = bound + 2.0 ** -25 * V.abs().sum(0)[None, :, None]
+                bound = bound + 2.0 ** -25 * (1 + V.abs().sum(0)[None, :, None])
             got = out[rows].double().view(t, self.HKV, G, D)
             bad = ~((got - ref).abs() <= bound)
             assert not bad.any(), (b, bad.sum().item(), (got - ref).abs().max().item(),
@@ -308,7 +309,7 @@ def test_decode_one_sequence(cuda, krlib, ctx, HQ, HKV, D):
 def test_tree(cuda, krlib, T, HQ, HKV, D, dtype):
     """Trees of drafted tokens at every offset of the draft inside a block and a mask word."""
     import torch
-    seqs = [(0, T), (5, T), (64 - T % 64, T), (127, T), (333, max(1, T - 1)), (1, 1), (990, T)]
+    seqs = [(0, T), (5, T), (64 - T % 64, T), (127, T), (77, 0), (333, max(1, T - 1)), (1, 1), (990, T)]
     b = Batch(seqs, HQ, HKV, D, 16, dtype, "nhd", masked=True, seed=T, empty={0, T // 2})
     out = b.run(krlib)
     torch.cuda.synchronize()
