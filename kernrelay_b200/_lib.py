@@ -353,7 +353,7 @@ def _is(t, dtype, index, dim):
     operators' smallest calls take a few microseconds, so their checks are kept as cheap (row
     pitches below: rows that are never stepped over may have any stride)."""
     return (t.dtype is dtype and t.get_device() == index and t.dim() == dim
-            and (t.stride(-1) == 1 or t.size(-1) <= 1))
+            and (t.stride()[-1] == 1 or t.shape[-1] <= 1))
 
 
 def _refuse(what, name, t, dtype, dim):
@@ -412,7 +412,7 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
             return qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm, k_norm,
                                       eps, layer, out, status, stream)
     if out is None:
-        out = _empty((N, HQ * D), dt, qkv, stream)
+        out = qkv.new_empty((N, HQ * D)) if stream is None else _empty((N, HQ * D), dt, qkv, stream)
     many = N > 1
     check(lib().krb_qk_norm_rope_paged(
         cache.ref, layer, qkv.data_ptr(), qkv.stride(0) if many else width, out.data_ptr(),
