@@ -68,6 +68,7 @@ struct AppendArgs {
   int N, HQ, HKV, max_pos, page_shift;
   int64_t total_slots;
   float eps;
+  bool stream_out;
   uint32_t *status;
 };
 
@@ -108,18 +109,18 @@ __device__ __forceinline__ uint4 ldg4(const void *p) {
 // in fp32 from the stored values to the one rounding of the store.
 //
 // Bound: HBM at size (every value read and written once), a launch when small.  What it takes is
-// loads in flight, and that is warps: the halves are rotated one after the other so that five CTAs
-// are resident, in paired fp32 (5 / 6 by the register limit: 42.7 / 42.9 us for 8192 tokens of 32 + 2
-// x 8 heads of 128 with norms, 203 MB, 31.6 us at the copy's rate; 8.3 / 8.3 for 8192 tokens of 14 + 2
-// x 2 heads of 64; unpaired 48.8 / 44.2 / 45.6 with 4 / 5 / 6).  Tried: several heads per warp with the
-// table products in registers (54 us, 14.5), and whole rows by bulk copies into shared memory (42.2
-// us, but 17.1).
+// loads in flight, and that is warps: the halves are rotated one after the other, in paired fp32, so
+// that forty warps are resident, and the rows, read once, leave L1 to the tables.  Measured: 8192
+// tokens of 32 + 2 x 8 heads of 128 with norms, 203 MB, 38.1 us, 0.83 of the copy's rate (rows
+// through L1 42.7; unpaired and 32 / 40 / 48 warps 48.8 / 44.2 / 45.6); 2400 of them 10.8 us, 0.87.
+// Tried: several heads per warp with the table products in registers (54 us), whole rows by bulk copies
+// into shared memory (42.2 us, and twice the time at 14 + 2 x 2 heads of 64).
 template <int D, bool F16>
-__global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(128, 10) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
   constexpr int kLanes = HALF / 8;
   pdl_wait();
-  const uint32_t gt = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t gt = blockIdx.x * 128u + threadIdx.x;
   const uint32_t nh = a.HQ + 2 * a.HKV;
   const uint32_t item = gt / kLanes;
   const int j = static_cast<int>(gt % kLanes) * 8;
@@ -127,13 +128,17 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
   if (n >= a.N) return;  // whole heads only
   const int h = static_cast<int>(item - n * nh);
   const uint16_t *p = a.qkv + n * a.ldqkv + h * D + j;
-  // plain loads: q_out may be the q columns of qkv
-  const uint4 wlo = *reinterpret_cast<const uint4 *>(p);
-  const uint4 whi = *reinterpret_cast<const uint4 *>(p + HALF);
+  // read once: kept out of the way of the tables (coherent loads: q_out may be the q columns of qkv)
+  const uint4 wlo = __ldcs(reinterpret_cast<const uint4 *>(p));
+  const uint4 whi = __ldcs(reinterpret_cast<const uint4 *>(p + HALF));
   const int64_t pos = a.positions[n];
   const bool pos_ok = pos >= 0 && pos < a.max_pos;
   if (!pos_ok && h == 0 && j == 0) report_status(a.status, kStatusBadIndex);
 
+  auto store = [&](uint16_t *to, const uint4 &w) {
+    if (a.stream_out) __stcs(reinterpret_cast<uint4 *>(to), w);
+    else *reinterpret_cast<uint4 *>(to) = w;
+  };
   uint16_t *dst;
   if (h < a.HQ) {
     dst = a.q_out + n * a.ldq + h * D + j;
@@ -149,8 +154,8 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
       dst = a.k + page * a.k_page + (h - a.HQ) * a.k_head + off * a.k_slot + j;
     } else {
       dst = a.v + page * a.v_page + (h - a.HQ - a.HKV) * a.v_head + off * a.v_slot + j;
-      *reinterpret_cast<uint4 *>(dst) = wlo;
-      *reinterpret_cast<uint4 *>(dst + HALF) = whi;
+      store(dst, wlo);
+      store(dst + HALF, whi);
       return;
     }
   }
@@ -193,21 +198,21 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const AppendArgs a) {
                             ts0.w ^ 0x80008000u), f);  // -sin
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = fma_f32x2(hi[e], f[e], y[e]);
-  *reinterpret_cast<uint4 *>(dst) = pack8<F16>(y);
+  store(dst, pack8<F16>(y));
   unpack8<false>(tc1, f);
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = mul_f32x2(hi[e], f[e]);
   unpack8<false>(ts1, f);
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = fma_f32x2(lo[e], f[e], y[e]);
-  *reinterpret_cast<uint4 *>(dst + HALF) = pack8<F16>(y);
+  store(dst + HALF, pack8<F16>(y));
 }
 
 template <int D, bool F16>
 void launch_append(const AppendArgs &a, cudaStream_t stream) {
   const long threads = static_cast<long>(a.N) * (a.HQ + 2 * a.HKV) * (D / 16);
   if (threads > 0xffffff00L) throw CudaError("qk_norm_rope_paged: too many tokens");
-  launch_pdl(append_kernel<D, F16>, dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0, stream, false, a);
+  launch_pdl(append_kernel<D, F16>, dim3(static_cast<unsigned>((threads + 127) / 128)), 128, 0, stream, false, a);
 }
 
 // ------------------------------------------------------------------ page copies
@@ -391,6 +396,10 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
   a.total_slots = int64_t(c.pages) * c.page_size;
   a.eps = eps;
   a.status = status;
+  // Output that the next kernel would not find in L2 (126 MB) as a whole goes past it: 42.1 -> 38.1 us
+  // for 101 MB (8192 tokens of 32 + 2 x 8 heads of 128); at 50 MB it would gain a twentieth and cost
+  // the reader.
+  a.stream_out = static_cast<int64_t>(N) * nh * D * 2 > (int64_t(64) << 20);
   if (D == 128 && c.dtype) launch_append<128, true>(a, stream);
   else if (D == 128) launch_append<128, false>(a, stream);
   else if (c.dtype) launch_append<64, true>(a, stream);

@@ -80,6 +80,7 @@ def _append_ref(x, w, cos, sin):
     (130, 4, 4, 64, 32, True, "fp16", "padded"),
     (1025, 14, 2, 64, 128, True, "bf16", "hnd"),
     (64, 4, 1, 128, 1024, False, "fp16", "hnd"),
+    (6001, 32, 8, 128, 64, True, "bf16", "hnd"),  # 74 MB: stored past L2
 ])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_append(cuda, krlib, n, HQ, HKV, D, page, norm, dtype, layout, in_place):
