@@ -201,5 +201,8 @@ def test_wrapper_refusals(krlib):
             krlib.kv_commit(c, **{**good, **over})
     with pytest.raises(krlib.KrbError, match="length"):
         krlib.kv_copy_pages(c, [1, 2], [3])
-    with pytest.raises(krlib.KrbError, match="host integers"):
-        krlib.kv_copy_pages(c, [1.5], [3])
+    for bad in (1.5, 2 ** 32 + 1, "1", None):
+        with pytest.raises(krlib.KrbError, match="host integers"):
+            krlib.kv_copy_pages(c, [bad], [3])
+    with pytest.raises(krlib.KrbError, match="not on a GPU"):
+        krlib.kv_copy_pages(c, [1], [3])

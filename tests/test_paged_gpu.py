@@ -569,6 +569,33 @@ def test_graph_follows_lengths(cuda, krlib):
         short.check(out)
 
 
+def test_two_graphs_at_once(cuda, krlib):
+    """Two captured calls replayed on two streams at a time: neither uses the other's workspace."""
+    import torch
+    bs = [Batch([(2000 + 700 * i, 1 + 20 * i), (55, 1)], 28, 4, 128, 16, seed=20 + i) for i in range(2)]
+    want = [b.run(krlib).clone() for b in bs]
+    outs = [torch.empty_like(w) for w in want]
+    caches = [krlib.KVCache(b.k, b.v) for b in bs]
+    status = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in bs]
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in bs]
+    for b, o, c, st in zip(bs, outs, caches, status):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            krlib.attention_paged(b.q, c, b.table, b.lens, b.starts, b.max_q, b.scale, out=o, status=st)
+    for _ in range(10):
+        for o in outs:
+            o.fill_(5.0)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for w, o, b in zip(want, outs, bs):
+            assert torch.equal(w[:b.starts_host[-1]], o[:b.starts_host[-1]])
+
+
 def test_same_result_twice(cuda, krlib):
     import torch
     b = Batch([(5000, 1), (77, 1), (2500, 1)], 28, 4, 128, 16, seed=4)
@@ -703,6 +730,63 @@ def test_commit_refuses_per_sequence(cuda, krlib):
     assert torch.equal(k[:, 4:], k0[:, 4:])
     flat0, flat = (x[:, :4].transpose(2, 3).reshape(2, -1, 2, 64) for x in (k0, k))
     assert torch.equal(flat[:, 6], flat0[:, 7]) and torch.equal(flat[:, 7], flat0[:, 10])
+
+
+# ---------------------------------------------------------------- large caches and batches
+@pytest.mark.parametrize("T", [1, 9])
+def test_past_32_bits(cuda, krlib, T):
+    """A cache of more than 2^31 elements: every operator on its last pages does what it does in a
+    small cache, bit for bit."""
+    import torch
+    HQ, HKV, D, page, n = 16, 8, 128, 64, 600
+    dt, g = torch.bfloat16, _gen(T)
+    most = 2 ** 31 // (HKV * page * D) + 1200
+    cos, sin = _rope_tables(n, D)
+    qkv = torch.randn(n, (HQ + 2 * HKV) * D, generator=g, device="cuda").to(dt)
+    pos = torch.arange(n, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    need = -(-n // page)
+    got = []
+    for pages, ids in ((need + 1, list(range(need + 1))),
+                       (most, [most - 1 - 7 * i for i in range(need - 1)] + [3, most - 3])):
+        k, v = (torch.empty(pages, HKV, page, D, dtype=dt, device="cuda") for _ in range(2))
+        cache = krlib.KVCache(k, v)
+        slots = torch.tensor(ids, device="cuda")[pos // page] * page + pos % page
+        q = krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        args = (i32([ids[:need]]), i32([n]), i32([0, T]), T, D ** -0.5)
+        first = krlib.attention_paged(q[n - T:], cache, *args, status=status)
+        krlib.kv_copy_pages(cache, [ids[0]], [ids[need]])
+        krlib.kv_commit(cache, args[0], i32([n - 80]), i32([[1, 4, 70]]), i32([3]), status=status)
+        last = krlib.attention_paged(q[n - T:], cache, *args, status=status)
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        got.append([q, first, last, k[ids[need]].clone(), v[ids[need]].clone(), k[ids[0]].clone()])
+        del k, v, cache
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert not torch.equal(got[0][1], got[0][2])  # the commit moved rows that are attended to
+    torch.cuda.empty_cache()
+
+
+def test_thousands_of_sequences(cuda, krlib):
+    import torch
+    rng = random.Random(3)
+    b = Batch([(rng.choice([0, 1, 7, 30]), rng.choice([0, 1, 1])) for _ in range(3001)], 4, 2, 64, 8, seed=3)
+    out = b.run(krlib)
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    b.check(out)
+
+
+def test_long_chunk(cuda, krlib):
+    """Thousands of new tokens in one sequence: hundreds of units of its own."""
+    import torch
+    b = Batch([(100, 5000), (9, 2)], 8, 2, 64, 64, "fp16", seed=8)
+    out = b.run(krlib)
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    b.check(out)
 
 
 # ---------------------------------------------------------------- together
