@@ -3,11 +3,12 @@
 //
 // Few rows are bound by reading K and V once: a 64-key block of one KV head is 32 KB at head_dim 128,
 // 0.75 us of one SM's share of HBM bandwidth, against 0.14 us of mma.sync for a 16-row tile.  So the
-// kernel is a ring of TMA loads (two CTAs of three 32 KB stages per SM, three times the bytes that
-// latency needs in flight), the rows of all query heads that share a KV head go through the tensor
-// cores together, and the four warps of a CTA split the keys, so that a block costs each a quarter.
+// kernel is a ring of TMA loads (two CTAs of two 32 KB stages per SM; a third only deepens the queue
+// at the memory, which then serves the SMs less evenly: 110.6 us against 108.3 in the first case
+// below), the rows of all query heads that share a KV head go through the tensor cores together, and
+// the four warps of a CTA split the keys, so that a block costs each a quarter.
 // Measured: 64 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads of 128,
-// 111 us, 92 % of what 659 MB take at the copy's rate; 2 sequences of 98 and 131 thousand, 80 us, 91 %.
+// 104.6 us, 98 % of what 659 MB take at the copy's rate; 2 sequences of 98 and 131 thousand, 76 us, 95 %.
 #include <algorithm>
 #include <string>
 
@@ -26,7 +27,7 @@ template <int D>
 struct Cfg {
   static constexpr int kHalf = kKeys * 128;             // 64 keys x 64 elements, bytes
   static constexpr int kTile = kKeys * D * 2;           // K or V block
-  static constexpr int kStages = D == 128 ? 3 : 6;      // 96 KB of ring
+  static constexpr int kStages = D == 128 ? 2 : 4;      // 64 KB of ring: see the top
   static constexpr int kMergeLane = D / 16 * 4 + 4;     // floats per lane: half of O, m and l
   static constexpr int kMerge = kMergeLane * 32 * 4;    // bytes per sending warp
   static constexpr int kBars = 2 * kStages * 8;
@@ -119,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int box = 1 << box_shift;
     const uint32_t box_bytes = box * 128;
     PageFeed feed;
+    const uint64_t policy = p.kv_once ? l2_policy_evict_first() : l2_policy_evict_normal();
     int n = 0;  // blocks issued
     bool ok = true;
     while (w.pos < w.end && ok) {
@@ -145,8 +147,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (lead) {
 #pragma unroll
             for (int half = 0; half < D / 64; ++half) {
-              tma_load_4d(to + half * C::kHalf, &tm_k, &full[s], half * 64, slot, w.h, page);
-              tma_load_4d(to + C::kTile + half * C::kHalf, &tm_v, &full[s], half * 64, slot, w.h, page);
+              tma_load_4d_hint(to + half * C::kHalf, &tm_k, &full[s], half * 64, slot, w.h, page,
+                               policy);
+              tma_load_4d_hint(to + C::kTile + half * C::kHalf, &tm_v, &full[s], half * 64, slot, w.h, page,
+                               policy);
             }
           }
         }
@@ -679,6 +683,11 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   p.tpt = pl.tpt;
   p.tile_tok = pl.tile_tok;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  // One unit reads a sequence's keys of a head, and a layer's cache does not stay in L2 (126 MB) from
+  // call to call: 64 decoding sequences 108.1 -> 104.6 us, 2 long ones 77.5 -> 76.1; with the first 32
+  // pages shared by all sequences still 100.2 -> 96.8 (wide trees, whose units share keys, gained nothing).
+  p.kv_once = a.max_q <= pl.tpt &&
+              4.0 * c.pages * c.page_size * c.heads * c.head_dim > double(int64_t(126) << 20);
   p.status = a.status;
   carve_workspace(p, pl.ctas, a.workspace);
 

@@ -16,7 +16,9 @@
 // A piece's start and end (first scores, last product, O out) cost some 5000 more.
 // Measured: 64-token trees (8 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads
 // of 128) 62 us, 0.32 of their flop at the library's rate; two chunks of 1024 tokens over 1 and
-// 8 thousand positions 187 us, 0.44; 8-token trees (32 rows, 169 MB) 40 us, 0.65 of the copy's rate.
+// 8 thousand positions 187 us, 0.44; 8-token trees (32 rows, 169 MB) 37 us, 0.70 of the copy's rate,
+// 64 sequences of them 117 us, 0.89.  With one tile a ring of 8 blocks is as good as 12 or better (38.1 us
+// against 39.1, without the L2 hint): a deeper queue serves the SMs less evenly.
 // Tried, the trees' and the chunks' time: 128-key blocks with one S stage (70, 205: the chain softmax
 // -> PV -> QK), these with half blocks of P (69, 201) and an issuer per tile (79, 215); one issuer for
 // all products on two stages (83, 239); QK issuers per tile on two stages (69, 203).
@@ -44,7 +46,7 @@ template <int D, int NT>
 struct Cfg {
   static constexpr int kQTile = 256 * D;       // bytes
   static constexpr int kTile = kKeys * D * 2;  // K or V block
-  static constexpr int kSlots = D == 64 ? 16 : (NT == 2 ? 10 : 12);
+  static constexpr int kSlots = D == 64 ? 16 : (NT == 2 ? 10 : 8);
   static constexpr int kThreads = 32 * kSoftmaxWarp + 128 * NT;
   static constexpr int kBars = 2 * kSlots + 2 + 6 * NT;
   static constexpr int kSmem =
@@ -272,6 +274,8 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
     const int box = 1 << box_shift;
     const uint32_t box_bytes = box * 128;
     PageFeed feed;
+    [[maybe_unused]] const uint64_t policy =
+        p.kv_once ? l2_policy_evict_first() : l2_policy_evict_normal();
     int base = 0, pieces = 0;  // ring index of the piece's first load
     int last = -1;             // ring index of this warp's last load
     bool ok = true;
@@ -314,8 +318,12 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
           if (lead) {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(ring + s * C::kTile + c * kChunk + i * box_bytes, map, &full[s], 64 * c, slot,
-                          w.h, page);
+              if constexpr (NT == 1)
+                tma_load_4d_hint(ring + s * C::kTile + c * kChunk + i * box_bytes, map, &full[s],
+                                 64 * c, slot, w.h, page, policy);
+              else
+                tma_load_4d(ring + s * C::kTile + c * kChunk + i * box_bytes, map, &full[s], 64 * c,
+                            slot, w.h, page);
           }
         }
         last = at;
