@@ -491,9 +491,12 @@ def kv_copy_pages(cache, src, dst, stream=None):
     if getattr(src, "is_cuda", False) or getattr(dst, "is_cuda", False):
         raise KrbError(f"{what}: src and dst must be host integers, not tensors on a GPU")
     try:
-        src, dst = (array("i", x.tolist() if hasattr(x, "tolist") else x) for x in (src, dst))
+        # through a list: array() takes bytes-like objects for memory of its entries
+        src, dst = (array("i", x.tolist() if hasattr(x, "tolist") else list(x)) for x in (src, dst))
     except (TypeError, OverflowError) as e:
         raise KrbError(f"{what}: src and dst must be host integers ({e})") from None
+    if len(src) != n or len(dst) != n:
+        raise KrbError(f"{what}: src and dst must be flat sequences of host integers")
     if (on := _enter(cache)) is not None:
         with on:
             return kv_copy_pages(cache, src, dst, stream)

@@ -206,3 +206,60 @@ def test_wrapper_refusals(krlib):
             krlib.kv_copy_pages(c, [bad], [3])
     with pytest.raises(krlib.KrbError, match="not on a GPU"):
         krlib.kv_copy_pages(c, [1], [3])
+
+
+@pytest.fixture
+def copied(krlib, monkeypatch):
+    """What kv_copy_pages hands to the library: (src, dst), n entries of each."""
+    calls = []
+
+    class Fake:
+        def krb_kv_copy_pages(self, cache, src, dst, n, stream):
+            calls.append(tuple(list((ctypes.c_int * n).from_address(x)) if n else [] for x in (src, dst)))
+            return 0
+
+    monkeypatch.setattr(krlib, "_enter", lambda cache: None)
+    monkeypatch.setattr(krlib, "_raw_stream", lambda stream, index: None)
+    monkeypatch.setattr(krlib, "lib", lambda: Fake())
+    return calls
+
+
+def test_copy_page_lists_of_every_kind(krlib, copied):
+    """Every host sequence of integers means its elements: bytes are page numbers up to 255, not memory
+    of four-byte entries."""
+    from array import array
+
+    import numpy as np
+    import torch
+    c = _cpu_cache(krlib)
+    kinds = [bytes, bytearray, memoryview, list, tuple, np.array, torch.tensor,
+             lambda x: array("q", x), lambda x: array("B", x), lambda x: np.array(x, dtype=np.uint8),
+             lambda x: range(x[0], x[-1] + 1)]
+    for kind in kinds:
+        values = [5, 6, 7, 8] if kind is kinds[-1] else [5, 0, 0, 1]
+        held = bytes(values) if kind is memoryview else values
+        copied.clear()
+        krlib.kv_copy_pages(c, kind(held), kind(held))
+        assert copied == [(values, values)], kind
+    copied.clear()
+    krlib.kv_copy_pages(c, b"\x05\x01\x02", (1, 2, 3))  # no multiple of four long
+    assert copied == [([5, 1, 2], [1, 2, 3])]
+
+
+def test_copy_page_lists_whose_length_lies(krlib, copied):
+    class Short(list):
+        def __len__(self):
+            return 9
+
+    class Long:
+        def __len__(self):
+            return 1
+
+        def tolist(self):
+            return [1, 2, 3]
+
+    c = _cpu_cache(krlib)
+    for x in (Short([1, 2]), Long()):
+        with pytest.raises(krlib.KrbError, match="flat sequences"):
+            krlib.kv_copy_pages(c, x, x)
+    assert copied == []
