@@ -319,9 +319,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             o[d][3] *= alpha[1];
           }
         }
-        // P enters the second product in the cache's type (its relative rounding, 2^-9 or 2^-12,
-        // is that of the output); the row sum takes the fp32 values
+        // P enters the second product in the cache's type, rounded by up to 2^-9 (bf16) or 2^-12
+        // (fp16) of itself; a row's largest is a power of two, so exact.  The row sum takes the
+        // fp32 values.
         uint32_t pf[NT / 2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) off[x] -= p_shift<F16, 0>();
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll

@@ -283,6 +283,16 @@ __device__ __forceinline__ float *slot_o(const Params &p, int cta, int slot) {
   return p.o + (static_cast<long>(cta) * 2 + slot) * p.rows * p.D;
 }
 
+// P goes into PV in the cache's type, as 2^(s - m + shift) of a row whose offset m lags its maximum by
+// at most LAG: fp16 starts losing bits at 2^-14, and many keys that small may outweigh the largest
+// one, so P uses the type up to 2^15 (m and the sums of all pieces carry the same factor, which the
+// division by the row sum takes out).  What is left below: a key's absolute error is 2^-25 of values
+// whose largest is 2^(15 - LAG) or more.  bf16 has the exponents of fp32 and needs no shift.
+template <bool F16, int LAG>
+__device__ __forceinline__ constexpr float p_shift() {
+  return F16 ? 15.f - LAG : 0.f;
+}
+
 __device__ __forceinline__ float exp2_mufu(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -39,8 +39,8 @@ constexpr uint32_t kChunk = kKeys * 128;  // a block's keys x 64 elements, bytes
 constexpr int kSoftmaxWarp = 4;           // warps 0: Q and K, 3: V, 1: QK, 2: PV, 4 ..: softmax
 constexpr uint32_t kTmemCols = 512;
 // The running offset of a row moves (and O is rescaled) only when its maximum grew by more than
-// 2^8: until then P <= 256, which both 2-byte types hold with their full precision.
-constexpr float kRescaleLog2 = 8.0f;
+// 2^8: P is at most 2^8 in bf16, 2^15 in fp16.
+constexpr int kRescaleLog2 = 8;
 
 template <int D, int NT>
 struct Cfg {
@@ -132,8 +132,9 @@ __device__ __forceinline__ float exp_block(const uint32_t (&s)[2][32], float sca
     const uint64_t x = pack_f32x2(s[e >> 4][(2 * e) & 31], s[e >> 4][(2 * e + 1) & 31]);
     const float2 a = unpack_f32x2(fma_f32x2(x, sc, mo));
     const float p0 = exp2_mufu(a.x), p1 = exp2_mufu(a.y);
-    // P in the cache's type (its rounding is that of the output); the row sum takes the fp32 values
-    // (the rounded ones gave the same error for a tenth more time)
+    // P in the cache's type, rounded by up to 2^-9 (bf16) or 2^-12 (fp16) of itself, the largest one
+    // too where the offset lags; the row sum takes the fp32 values (the rounded ones gave the same
+    // error for a tenth more time)
     pk[e] = pack2<F16>(p0, p1);
     sum[e & 3] = add_f32x2(sum[e & 3], pack_f32x2(__float_as_uint(p0), __float_as_uint(p1)));
   }
@@ -142,8 +143,8 @@ __device__ __forceinline__ float exp_block(const uint32_t (&s)[2][32], float sca
 }
 
 // A block of one row: S (64 columns at s_col) -> P over its first 32 columns.  `see`(c): which of
-// the 32 keys of half c the row sees.  P = 2^(s * scale - m) with the row's offset m, which moves
-// only by more than kRescaleLog2; O and l follow it.  Behind a piece's first block (`has_o`) the
+// the 32 keys of half c the row sees.  P = 2^(s * scale - m + shift) with the row's offset m, which
+// moves only by more than kRescaleLog2; O and l follow it.  Behind a piece's first block (`has_o`) the
 // exponentials do not wait for the maximum: they are taken with the old m, and once more where it
 // moves, which is rare.  A row that has seen nothing yet has m = -inf and takes the offset 0.  `o_ready`
 // waits until no product writes O.
@@ -164,9 +165,10 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
         if (!((bits >> e) & 1)) r[c][e] = 0xff800000u;  // -inf
     }
   }
+  constexpr float shift = p_shift<F16, kRescaleLog2>();
   uint32_t pk[32];
   float sum = 0.f;
-  if (has_o) sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
+  if (has_o) sum = exp_block<F16>(r, scale_log2, (m_run == -INFINITY ? 0.f : m_run) - shift, pk);
   float m4[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) m4[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
@@ -178,7 +180,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
   if (!has_o || __any_sync(0xffffffffu, grow)) {
     const float alpha = grow ? exp2_mufu(m_run - top) : 1.f;
     if (grow) m_run = top;
-    sum = exp_block<F16>(r, scale_log2, m_run == -INFINITY ? 0.f : m_run, pk);
+    sum = exp_block<F16>(r, scale_log2, (m_run == -INFINITY ? 0.f : m_run) - shift, pk);
     l_run *= alpha;
     if (has_o) {
       o_ready();

@@ -870,3 +870,41 @@ def test_draft_verify_commit(cuda, krlib, HQ, HKV, D, dtype):
                         for j in paths[b]]
         krlib.kv_commit(cache, i32(table), i32(lens), acc.cuda(), i32([len(p) for p in paths]))
         lens = [n + len(p) for n, p in zip(lens, paths)]
+
+
+# ---------------------------------------------------------------- small probabilities
+@pytest.mark.parametrize("T", [1, 8, 40])
+@pytest.mark.parametrize("HQ,HKV,D", [(28, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("fall", [(15.0, 15.0), (24.875, 24.875), (25.125, 25.125), (14.0, 30.0)])
+def test_small_probabilities_count_in_fp16(cuda, krlib, T, HQ, HKV, D, fall):
+    """One key far above all others, whose value is zero: the output is what the thousands of small
+    probabilities add up to, 2^-14 to 2^-30 of the largest each (below fp16's normal numbers).  Bound:
+    that of the attention tests with a probability's absolute error 2^-25 relative to the largest
+    one's power of two, which is 2^15 or, behind an offset that lags by up to 8, 2^7."""
+    import torch
+    B, n, page = 128, 16384, 64  # units enough that most lie whole in a CTA, the largest key with them
+    u = 2.0 ** -11
+    g = _gen(T)
+    x = torch.linspace(*fall, n, device="cuda")  # log2 of how far a key is below the first
+    x[0] = 0
+    k = torch.zeros(1, n // page, HKV, page, D, dtype=torch.float16, device="cuda")
+    v = torch.rand(k.shape, generator=g, device="cuda").add_(0.5).half()
+    k[0, ..., 0] = (-x / 8).half().view(n // page, 1, page)
+    v[0, 0, :, 0] = 0
+    q = torch.zeros(B * T, HQ, D, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").repeat(B, 1)
+    mask = torch.full((B * T, 2), -1, dtype=torch.int32, device="cuda")  # every row sees every key
+    out = krlib.attention_paged(q.view(B * T, -1), krlib.KVCache(k, v), table, i32([n] * B),
+                                i32([T * i for i in range(B + 1)]), T, math.log(2), mask=mask)
+    torch.cuda.synchronize()
+    K, V = (t[0].transpose(1, 2).reshape(n, HKV, D).double() for t in (k, v))
+    p = torch.softmax(K[:, 0, 0] * 8 * math.log(2), 0)
+    ref = torch.einsum("n,nhd->hd", p, V)
+    S = fall[1] * math.log(2)
+    rel = 2 * (D + 4) * 2.0 ** -24 * S + n * 2.0 ** -24 + 2.0 ** -20
+    bound = u * ref + (u + rel) * ref * (1 + 2 * u) + 2.0 ** -32 * V.sum(0) + 2.0 ** -25
+    got = out.double().view(B * T, HKV, HQ // HKV, D)
+    bad = ~((got - ref[None, :, None]).abs() <= bound[None, :, None])
+    assert not bad.any(), ((got - ref[None, :, None]) / ref[None, :, None]).abs().max().item()
