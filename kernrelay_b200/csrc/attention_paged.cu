@@ -132,11 +132,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int key0 = blk * kKeys;
         const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
         feed.advance(p, key0);
-        ok = mbar_wait(&empty[s], ((n / C::kStages) & 1) ^ 1, kMbarLimitNs);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        ok = mbar_wait_warp(&empty[s], ((n / C::kStages) & 1) ^ 1);
+        if (!ok) break;
         uint8_t *stage = smem + s * 2 * C::kTile;
         const bool lead = elect_one();
         if (lead) mbar_arrive_expect_tx(&full[s], nbox * box_bytes * (D / 64 * 2));
@@ -220,11 +217,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     for (int blk = vw->blk; blk < e; ++blk, ++n) {
       const int s = n % C::kStages;
-      if (ok) ok = mbar_wait(&full[s], (n / C::kStages) & 1, kMbarLimitNs);
-      if (!__all_sync(0xffffffffu, ok)) {  // leave the waits, keep the CTA's barriers in step
-        ok = false;
-        continue;
-      }
+      if (ok) ok = mbar_wait_warp(&full[s], (n / C::kStages) & 1);
+      if (!ok) continue;  // leave the waits, keep the CTA's barriers in step
       const int k0 = blk * kKeys + wn * kWarpKeys;  // this warp's first key
       const uint32_t kt = base + s * 2 * C::kTile, vt = kt + C::kTile;
       const bool wrote = k0 + kWarpKeys > end;

@@ -245,6 +245,13 @@ struct PageFeed {
   }
 };
 
+// A wait of a whole warp whose lanes go on together or not at all: a wait that ran out for some of
+// them may have come for the others at its last poll, and a lane that left alone would be missing
+// from the warp's next vote or tensor-memory access.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, kMbarLimitNs));
+}
+
 // one lane of a warp that is converged (the same one every time)
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;

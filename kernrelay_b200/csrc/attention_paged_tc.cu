@@ -147,7 +147,7 @@ __device__ __forceinline__ float exp_block(const uint32_t (&s)[2][32], float sca
 // moves only by more than kRescaleLog2; O and l follow it.  Behind a piece's first block (`has_o`) the
 // exponentials do not wait for the maximum: they are taken with the old m, and once more where it
 // moves, which is rare.  A row that has seen nothing yet has m = -inf and takes the offset 0.  `o_ready`
-// waits until no product writes O.
+// waits until no product writes O; where that wait runs out (false, for the warp), O is left alone.
 template <int D, bool F16, bool kMask, typename See, typename Ready>
 __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, float scale_log2,
                                              bool has_o, float &m_run, float &l_run, See see,
@@ -182,8 +182,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
     if (grow) m_run = top;
     sum = exp_block<F16>(r, scale_log2, (m_run == -INFINITY ? 0.f : m_run) - shift, pk);
     l_run *= alpha;
-    if (has_o) {
-      o_ready();
+    if (has_o && o_ready()) {
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
@@ -289,8 +288,7 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
       feed.begin(p, w.b, w.blk * kKeys, min(end, e * kKeys));
       if (!v) {
         const bool has_b = NT > 1 && tok0 + p.tile_tok < w.T;
-        ok = mbar_wait(q_empty, (pieces & 1) ^ 1, kMbarLimitNs);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = mbar_wait_warp(q_empty, (pieces & 1) ^ 1);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t bytes = p.tile_tok * p.group * D * 2;
@@ -308,8 +306,7 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
         const int key0 = (w.blk + j) * kKeys;
         const int nbox = (min(kKeys, end - key0) + box - 1) >> box_shift;
         feed.advance(p, key0);
-        ok = mbar_wait(&empty[s], ((at / C::kSlots) & 1) ^ 1, kMbarLimitNs);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = mbar_wait_warp(&empty[s], ((at / C::kSlots) & 1) ^ 1);
         if (!ok) break;
         const bool lead = elect_one();
         if (lead) mbar_arrive_expect_tx(&full[s], nbox * box_bytes * (D / 64));
@@ -392,11 +389,7 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
     int base = 0;
     uint32_t done[2] = {0, 0};
     bool ok = true;
-    auto wait = [&](uint64_t *bar, uint32_t parity) {
-      ok = mbar_wait(bar, parity, kMbarLimitNs);
-      ok = __all_sync(0xffffffffu, ok);
-      return ok;
-    };
+    auto wait = [&](uint64_t *bar, uint32_t parity) { return ok = mbar_wait_warp(bar, parity); };
     while (w.pos < w.end && ok) {
       const int e = piece_end(w);
       const int n = e - w.blk;
@@ -465,17 +458,17 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
         for (int j = 0; j < nblk && ok; ++j) {
           const int key0 = (w.blk + j) * kKeys;
           const int c = mine + j, stage = c & 1;  // blocks of this tile before this one
-          ok = mbar_wait(&s_full[2 * x + stage], (c >> 1) & 1, kMbarLimitNs);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
+          ok = mbar_wait_warp(&s_full[2 * x + stage], (c >> 1) & 1);
+          if (!ok) break;
           tc_fence_after();
           if (any_row) {
-            // PV of the block before (that of the one before it is complete: this S came after it)
+            // PV of the block before (that of the one before it is complete: this S came after it).
+            // Where it does not come, O stays untouched and the warp leaves after this block; nothing is
+            // stored.
             auto o_ready = [&] {
-              if (!mbar_wait(&o_done[2 * x + (stage ^ 1)], ((c - 1) >> 1) & 1, kMbarLimitNs)) ok = false;
+              ok = mbar_wait_warp(&o_done[2 * x + (stage ^ 1)], ((c - 1) >> 1) & 1);
               tc_fence_after();
+              return ok;
             };
             if (key0 + kKeys > hidden_from)
               softmax_block<D, F16, true>(
@@ -489,11 +482,8 @@ __global__ void __launch_bounds__(32 * kSoftmaxWarp + 128 * NT, 1)
           mbar_arrive(&p_ready[2 * x + stage]);
         }
         mine += nblk;
-        if (ok) ok = mbar_wait(&o_done[2 * x + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, kMbarLimitNs);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        if (ok) ok = mbar_wait_warp(&o_done[2 * x + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1);
+        if (!ok) break;
         tc_fence_after();
         if (any_row) {
           const bool whole = w.blk == 0 && e == w.nblk;

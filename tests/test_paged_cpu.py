@@ -263,3 +263,48 @@ def test_copy_page_lists_whose_length_lies(krlib, copied):
         with pytest.raises(krlib.KrbError, match="flat sequences"):
             krlib.kv_copy_pages(c, x, x)
     assert copied == []
+
+
+# ---------------------------------------------------------------- the kernels' error paths
+def _blocks(text, head):
+    """Spans of the brace blocks that `head` opens."""
+    at = 0
+    while (at := text.find(head, at)) >= 0:
+        depth, end = 1, at + len(head)
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        yield at, end
+        at += 1
+
+
+def bare_waits(text):
+    """Calls of mbar_wait whose outcome steers code that a whole warp runs."""
+    import re
+    text = re.sub(r"//[^\n]*", "", text)
+    single = list(_blocks(text, "if (lane == 0) {"))
+    found = []
+    for m in re.finditer(r"\bmbar_wait\(", text):
+        used = re.search(r"(return|[=(!&|,])\s*$", text[:m.start()])
+        if used and not any(a < m.start() < b for a, b in single):
+            found.append(text[m.start():text.index(";", m.start())])
+    return found
+
+
+def test_a_warp_leaves_its_waits_together():
+    """A wait that runs out does so lane by lane.  Where a warp goes on to votes, barriers or
+    tensor-memory accesses, its lanes decide together (mbar_wait_warp): one that left alone would
+    leave the others waiting for good.  (A wait cannot be made to run out on a GPU without a kernel
+    that is broken for it; the sources are what can be checked.)"""
+    from pathlib import Path
+    csrc = Path(__file__).resolve().parents[1] / "kernrelay_b200" / "csrc"
+    assert bare_waits("ok = mbar_wait(&a[b], 1, n);  // x\nif (ok) {}") == ["mbar_wait(&a[b], 1, n)"]
+    assert not bare_waits("if (lane == 0) { ok = mbar_wait(a, 1, n); }  for (;;) mbar_wait(a, 1, n);")
+    for name in ("attention_paged.cu", "attention_paged_tc.cu"):
+        text = (csrc / name).read_text()
+        assert bare_waits(text) == [], name
+        for a, b in _blocks(text, "if (lane == 0) {"):
+            assert "mbar_wait_warp" not in text[a:b]
+    head = (csrc / "attention_paged.cuh").read_text()
+    assert "return __all_sync(0xffffffffu, mbar_wait(bar, parity, kMbarLimitNs));" in head
+    assert len(bare_waits(head)) == 1
