@@ -131,7 +131,8 @@ typedef struct krb_kv_cache {
 /* Per token n of qkv [N, (HQ+2*HKV)*D] (cache dtype, row pitch ldqkv; HKV = heads, D =
  * head_dim): optional per-head RMSNorm of the q and k heads (q_norm / k_norm bf16 [D], both or
  * neither), rotate-half RoPE with row positions[n] of the bf16 tables cos / sin [max_pos, D],
- * then q -> q_out [N, HQ*D] (row pitch ldq; may be the q columns of qkv itself), and the k and
+ * then q -> q_out [N, HQ*D] (row pitch ldq; may be the q columns of qkv itself, and may not overlap
+ * qkv in any other way), and the k and
  * v heads -> slot slots[n] = page * page_size + offset of `layer`.  Rounds once, at the store.
  * slots[n] = -1 writes no k and v (a padded token); any other slots must differ from each
  * other.  A slot outside [-1, pages * page_size) sets bit 8 and writes no k and v; a position
@@ -158,7 +159,7 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * (So does, for the whole call, a sequence of more than 2^26 blocks of 64 keys, its row tiles and
  * KV heads counted each, or 2^31 in all.)
  * A page outside [0, pages) sets bit 8 and is read as page 0.
- * out must not overlap q.
+ * out may not overlap q (refused).
  * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call
  * alone until it is done; calls in order on one stream may share one. */
 int krb_attention_paged(const krb_kv_cache *cache, int layer, const void *q, int64_t ldq,

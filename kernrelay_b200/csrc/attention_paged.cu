@@ -648,6 +648,8 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   if (!(a.scale > 0.f) || a.scale > 1e30f) throw CudaError("attention_paged: scale must be positive");
   if (a.mask && (a.mask_words <= 0 || a.ldm < a.mask_words || long(a.mask_words) * 32 < a.max_q))
     throw CudaError("attention_paged: mask rows narrower than max_q");
+  if (rows_overlap(a.q, a.ldq, width, a.out, a.ldo, width, a.N))
+    throw CudaError("attention_paged: out overlaps q");
   int device = 0;
   KRB_CUDA(cudaGetDevice(&device));
   const Plan pl = plan_of(group, a.max_q, c.head_dim, device);

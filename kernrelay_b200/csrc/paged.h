@@ -34,6 +34,10 @@ void launch_pdl(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream
 // rows overlap); `layer` in [0, layers).
 void check_cache(const krb_kv_cache *c, int layer, const char *what);
 
+// Whether any of n rows of `wa` 2-byte elements at pitch `la` shares an element with any of n rows
+// of `wb` at pitch `lb` (pitches no smaller than their rows).
+bool rows_overlap(const void *a, long la, long wa, const void *b, long lb, long wb, int n);
+
 struct PagedAttnArgs {
   const void *q;
   long ldq;

@@ -47,6 +47,25 @@ void check_cache(const krb_kv_cache *c, int layer, const char *what) {
   check_strides(c->v_stride, *c, what);
 }
 
+bool rows_overlap(const void *a, long la, long wa, const void *b, long lb, long wb, int n) {
+  using i128 = __int128;  // pitches are the caller's
+  const i128 a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  const i128 pa = i128(la) * 2, pb = i128(lb) * 2, ra = i128(wa) * 2, rb = i128(wb) * 2;
+  const i128 last = n - 1;
+  if (a0 + last * pa + ra <= b0 || b0 + last * pb + rb <= a0) return false;
+  if (n > 1 && pa == pb) {  // columns of one buffer, maybe
+    const i128 d = ((b0 - a0) % pa + pa) % pa;
+    return d < ra || d + rb > pa;
+  }
+  for (i128 i = 0, j = 0; i < n && j < n;) {
+    const i128 ea = a0 + i * pa + ra, eb = b0 + j * pb + rb;
+    if (ea - ra < eb && eb - rb < ea) return true;
+    if (ea <= eb) ++i;
+    else ++j;
+  }
+  return false;
+}
+
 namespace {
 
 int ilog2(int v) {
@@ -369,6 +388,9 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
                         static_cast<const void *>(k_norm)})
     if (reinterpret_cast<uintptr_t>(p) % 16)
       throw CudaError("qk_norm_rope_paged: pointers must be 16-byte aligned");
+  if (!(q_out == qkv && (ldq == ldqkv || N == 1)) &&
+      rows_overlap(qkv, ldqkv, static_cast<long>(nh) * D, q_out, ldq, static_cast<long>(HQ) * D, N))
+    throw CudaError("qk_norm_rope_paged: q_out overlaps qkv, and is not its q columns");
   AppendArgs a{};
   a.qkv = static_cast<const uint16_t *>(qkv);
   a.ldqkv = ldqkv;

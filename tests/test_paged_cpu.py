@@ -308,3 +308,50 @@ def test_a_warp_leaves_its_waits_together():
     head = (csrc / "attention_paged.cuh").read_text()
     assert "return __all_sync(0xffffffffu, mbar_wait(bar, parity, kMbarLimitNs));" in head
     assert len(bare_waits(head)) == 1
+
+
+# ---------------------------------------------------------------- outputs over inputs
+W, W3 = 28 * 128, 36 * 128  # q's columns, and qkv's, of the calls above
+
+
+@pytest.mark.parametrize("at,ldo,N,free", [
+    (0, W, 3, False), (0, W, 1, False), (8, W, 1, False), (W - 8, W, 1, False), (W, W, 1, True),
+    (2 * W, W, 3, False), (3 * W, W, 3, True), (-3 * W, W, 3, True), (-3 * W + 8, W, 3, False),
+    (-W, W, 1, True), (W, 3 * W, 3, False), (2 * W, 2 * W + 8, 3, False), (-W, W + 8, 2, False),
+])
+def test_attention_output_over_q(krlib, at, ldo, N, free):
+    """Rows of q (dense, at 1 << 30) and out at every way of touching.  No workspace is given, so that
+    what is not refused for its overlap is refused behind it."""
+    d, base = _desc(krlib), 1 << 30
+    rc = krlib.lib().krb_attention_paged(
+        ctypes.addressof(d), 0, base, W, base + 2 * at, ldo, N, 28, 16, 8, 8, 16, 16, 2, 1, None, 0, 0,
+        0.1, None, 0, None, None)
+    assert rc == 1
+    assert ("out overlaps q" in _message(krlib)) == (not free)
+
+
+@pytest.mark.parametrize("at,lda,ldo,free", [
+    (W, 2 * W, 2 * W, True), (W - 8, 2 * W, 2 * W, False), (W + 8, 2 * W, 2 * W, False),
+    (W + 8, 2 * W + 8, 2 * W + 8, True), (-W, 2 * W, 2 * W, True), (W, 4 * W, 2 * W, True),
+    (W, 4 * W, 2 * W + 8, False), (3 * W, 4 * W, 4 * W, True), (3 * W + 8, 4 * W, 4 * W, False),
+])
+def test_attention_output_beside_q(krlib, at, lda, ldo, free):
+    """Columns of one buffer: rows that lie between each other without sharing an element are taken."""
+    d, base = _desc(krlib), 1 << 30
+    rc = krlib.lib().krb_attention_paged(
+        ctypes.addressof(d), 0, base, lda, base + 2 * at, ldo, 50, 28, 16, 8, 8, 16, 16, 2, 1, None, 0, 0,
+        0.1, None, 0, None, None)
+    assert rc == 1
+    assert ("out overlaps q" in _message(krlib)) == (not free)
+    brute = any(abs(at + j * ldo - i * lda) < W for i in range(50) for j in range(50))
+    assert brute == (not free)
+
+
+@pytest.mark.parametrize("at,ldq,N", [(8, W3, 3), (0, W, 3), (W, W3, 3), (8 * 128, W, 2), (W3 - 8, W, 1),
+                                      (-8, W, 1), (-3 * W + 8, W, 3)])
+def test_append_output_over_qkv(krlib, at, ldq, N):
+    d, base = _desc(krlib), 1 << 30
+    rc = krlib.lib().krb_qk_norm_rope_paged(
+        ctypes.addressof(d), 0, base, W3, base + 2 * at, ldq, 16, 16, N, 28, 16, 16, 8, None, None, 1e-6,
+        None, None)
+    assert rc == 1 and "overlaps qkv" in _message(krlib)

@@ -908,3 +908,41 @@ def test_small_probabilities_count_in_fp16(cuda, krlib, T, HQ, HKV, D, fall):
     got = out.double().view(B * T, HKV, HQ // HKV, D)
     bad = ~((got - ref[None, :, None]).abs() <= bound[None, :, None])
     assert not bad.any(), ((got - ref[None, :, None]) / ref[None, :, None]).abs().max().item()
+
+
+# ---------------------------------------------------------------- outputs beside inputs
+@pytest.mark.parametrize("T", [1, 40])
+def test_outputs_between_input_rows(cuda, krlib, T):
+    """q, qkv and outputs as columns of one buffer, of equal and of different pitches, overlap in no
+    element: they are taken, and give what apart from each other they give."""
+    import torch
+    b = Batch([(70, T), (9, T)], 8, 2, 64, 16, seed=T)
+    want = b.run(krlib)
+    N, w = b.q.shape
+    for lda, at, ldo in ((3 * w, w, 3 * w), (4 * w, w, 2 * w), (2 * w + 8, w + 8, 2 * w + 8)):
+        flat = torch.full((N * 4 * w,), 5.0, dtype=b.dt, device="cuda")
+        q = flat.as_strided((N, w), (lda, 1))
+        q.copy_(b.q)
+        out = flat.as_strided((N, w), (ldo, 1), at)
+        out.fill_(5.0)
+        keep, b.q = b.q, q
+        got = b.run(krlib, out=out)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(q, keep)
+        b.q = keep
+    HQ, HKV, D = 8, 2, 64
+    wide = torch.randn(N, 2 * (HQ + 2 * HKV) * D, generator=b.g, device="cuda").to(b.dt)
+    qkv, out = wide[:, :(HQ + 2 * HKV) * D], wide[:, (HQ + 2 * HKV) * D:][:, :HQ * D]
+    cos, sin = _rope_tables(64, D)
+    pos = torch.arange(N, device="cuda") % 64
+    slots = torch.full((N,), -1, device="cuda")
+    cache = krlib.KVCache(b.k, b.v)
+    want = krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin)
+    got = krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin, out=out)
+    assert torch.equal(got, want)
+    assert torch.equal(krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin, out=qkv[:, :HQ * D]),
+                       want)  # in place
+    with pytest.raises(krlib.KrbError, match="overlaps qkv"):
+        krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin, out=qkv[:, D:HQ * D + D])
+    with pytest.raises(krlib.KrbError, match="overlaps q"):
+        b.run(krlib, out=b.q)
