@@ -153,7 +153,8 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * tokens; needs max_q <= 32 * mask_words).  A row that sees nothing gives zeros.  The drafted
  * tokens' keys and values must be finite where other tokens of the sequence are to be (a masked
  * infinite value times a zero probability is not a number); slots behind kv_lens[b] may hold
- * anything.  max_q bounds every T_b, HQ / HKV <= 64, scale > 0.  T_b = 0 is allowed.
+ * anything.  max_q bounds every T_b (at least 1 where N and B are),
+ * HQ / HKV <= 64, scale > 0.  T_b = 0 is allowed.
  * A sequence with T_b > max_q, kv_lens[b] < T_b or > max_pages * page_size, or rows outside
  * [0, N) sets bit 7 and its rows are left as they were, like rows that belong to no sequence.
  * (So does, for the whole call, a sequence of more than 2^26 blocks of 64 keys, its row tiles and

@@ -466,7 +466,7 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
         with on:
             return attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask,
                                    layer, out, workspace, status, stream)
-    need = cache.attention_workspace(HQ, max_q)
+    need = cache.attention_workspace(HQ, max_q) if N and B else 0
     many = N > 1
     if out is None:
         out = torch.empty_like(q) if stream is None else _empty((N, width), dt, q, stream)

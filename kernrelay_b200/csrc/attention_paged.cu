@@ -613,7 +613,7 @@ static Plan plan_of(int group, int max_q, int D, int device) {
 static int group_of(const krb_kv_cache &c, int HQ, int max_q) {
   if (HQ <= 0 || HQ % c.heads) throw CudaError("attention_paged: HQ must be a multiple of the cache's heads");
   if (HQ / c.heads > 64) throw CudaError("attention_paged: more than 64 query heads per KV head");
-  if (max_q <= 0 || max_q > (1 << 24)) throw CudaError("attention_paged: bad max_q");
+  if (max_q < 0 || max_q > (1 << 24)) throw CudaError("attention_paged: bad max_q");
   return HQ / c.heads;
 }
 
@@ -623,7 +623,7 @@ size_t attention_paged_workspace(const krb_kv_cache &c, int HQ, int max_q) {
   const int group = paged::group_of(c, HQ, max_q);
   int device = 0;
   KRB_CUDA(cudaGetDevice(&device));
-  const paged::Plan pl = paged::plan_of(group, max_q, c.head_dim, device);
+  const paged::Plan pl = paged::plan_of(group, std::max(max_q, 1), c.head_dim, device);
   return paged::workspace_bytes(pl.ctas, pl.rows, c.head_dim);
 }
 
@@ -632,6 +632,7 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   if (a.N < 0 || a.B < 0) throw CudaError("attention_paged: negative size");
   const int group = group_of(c, a.HQ, a.max_q);
   if (a.N == 0 || a.B == 0) return;
+  if (a.max_q == 0) throw CudaError("attention_paged: bad max_q (0 with rows and sequences)");
   if (!a.q || !a.out || !a.page_table || !a.kv_lens || !a.q_starts)
     throw CudaError("attention_paged: null pointer");
   const long width = static_cast<long>(a.HQ) * c.head_dim;

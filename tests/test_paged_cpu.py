@@ -355,3 +355,15 @@ def test_append_output_over_qkv(krlib, at, ldq, N):
         ctypes.addressof(d), 0, base, W3, base + 2 * at, ldq, 16, 16, N, 28, 16, 16, 8, None, None, 1e-6,
         None, None)
     assert rc == 1 and "overlaps qkv" in _message(krlib)
+
+
+def test_attention_of_a_step_without_tokens(krlib):
+    """No rows or no sequences: nothing is done, and max_q, a bound of nothing, may be 0."""
+    d = ctypes.addressof(keep := _desc(krlib))
+    L = krlib.lib()
+    for N, B in ((0, 2), (3, 0), (0, 0)):
+        assert L.krb_attention_paged(d, 0, None, 0, None, 0, N, 28, None, 0, 0, None, None, B, 0, None, 0,
+                                     0, 0.1, None, 0, None, None) == 0
+        assert L.krb_attention_paged(d, 0, None, 0, None, 0, N, 28, None, 0, 0, None, None, B, -1, None, 0,
+                                     0, 0.1, None, 0, None, None) == 1 and "max_q" in _message(krlib)
+    del keep

@@ -946,3 +946,20 @@ def test_outputs_between_input_rows(cuda, krlib, T):
         krlib.qk_norm_rope_paged(qkv, cache, pos, slots, HQ, cos, sin, out=qkv[:, D:HQ * D + D])
     with pytest.raises(krlib.KrbError, match="overlaps q"):
         b.run(krlib, out=b.q)
+
+
+# ---------------------------------------------------------------- steps without tokens
+@pytest.mark.parametrize("max_q", [0, 1, 40])
+def test_attention_without_tokens(cuda, krlib, max_q):
+    import torch
+    k, v = _cache_tensors(1, 2, 2, 16, 64, torch.bfloat16, "hnd", fill=1.0)
+    cache = krlib.KVCache(k, v)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.empty(0, 8 * 64, dtype=torch.bfloat16, device="cuda")
+    assert krlib.attention_paged(q, cache, i32(3, 2), i32(3), i32(4), max_q, 0.1).shape == q.shape
+    assert krlib.attention_paged(q, cache, i32(0, 2), i32(0), i32(1), max_q, 0.1).shape == q.shape
+    out = torch.full((5, 8 * 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = krlib.attention_paged(torch.ones_like(out), cache, i32(0, 2), i32(0), i32(1), max_q, 0.1, out=out)
+    torch.cuda.synchronize()
+    assert (got == 5.0).all()  # rows of no sequence
+    assert cache.attention_workspace(8, 0) == cache.attention_workspace(8, 1) > 0
