@@ -403,8 +403,8 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
         _refuse(what, "q_norm [head_dim]", q_norm, bf, 1)
     if k_norm is not None and not (_is(k_norm, bf, index, 1) and k_norm.shape[0] == D):
         _refuse(what, "k_norm [head_dim]", k_norm, bf, 1)
-    if status is not None and not _is(status, torch.int32, index, 1):
-        _refuse(what, "status", status, torch.int32, 1)
+    if status is not None and not (_is(status, torch.int32, index, 1) and len(status)):
+        _refuse(what, "status [1]", status, torch.int32, 1)
     if out is not None and not (_is(out, dt, index, 2) and out.shape == (N, HQ * D)):
         _refuse(what, "out [N, HQ*head_dim]", out, dt, 2)
     if (on := _enter(cache)) is not None:
@@ -455,9 +455,11 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
         rows, words = mask.shape
         if rows != N:
             raise KrbError(f"{what}: mask must have one row per row of q")
+        if not words and N:  # a tensor without elements has no address: it would pass for no mask
+            raise KrbError(f"{what}: mask must have words of 32 bits for max_q tokens")
         ldm = mask.stride(0) if N > 1 else words
-    if status is not None and not _is(status, i32, index, 1):
-        _refuse(what, "status", status, i32, 1)
+    if status is not None and not (_is(status, i32, index, 1) and len(status)):
+        _refuse(what, "status [1]", status, i32, 1)
     if out is not None and not (_is(out, dt, index, 2) and out.shape == q.shape):
         _refuse(what, "out [N, HQ*head_dim]", out, dt, 2)
     if workspace is not None and not _is(workspace, torch.uint8, index, 1):
@@ -522,8 +524,8 @@ def kv_commit(cache, page_table, bases, accepted, counts, status=None, stream=No
     rows, max_pages = page_table.shape
     if rows != B or bases.shape[0] != B or counts.shape[0] != B:
         raise KrbError(f"{what}: page_table, bases, accepted and counts must be of the same batch")
-    if status is not None and not _is(status, i32, index, 1):
-        _refuse(what, "status", status, i32, 1)
+    if status is not None and not (_is(status, i32, index, 1) and len(status)):
+        _refuse(what, "status [1]", status, i32, 1)
     if (on := _enter(cache)) is not None:
         with on:
             return kv_commit(cache, page_table, bases, accepted, counts, status, stream)

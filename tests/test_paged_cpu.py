@@ -367,3 +367,24 @@ def test_attention_of_a_step_without_tokens(krlib):
         assert L.krb_attention_paged(d, 0, None, 0, None, 0, N, 28, None, 0, 0, None, None, B, -1, None, 0,
                                      0, 0.1, None, 0, None, None) == 1 and "max_q" in _message(krlib)
     del keep
+
+
+def test_masks_and_status_without_elements(krlib):
+    """A mask of no words is no mask's absence, and a status of no entries reports nothing: refused."""
+    import torch
+    c = _cpu_cache(krlib)
+    c._workspaces[4, 1] = 64
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    q, pos = torch.zeros(3, 4 * 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    good = dict(q=q, cache=c, page_table=i32(2, 4), kv_lens=i32(2), q_starts=i32(3), max_q=1, scale=0.1)
+    with pytest.raises(krlib.KrbError, match="mask must have words"):
+        krlib.attention_paged(**good, mask=i32(3, 0))
+    tab = torch.zeros(9, 64, dtype=torch.bfloat16)
+    for call in (lambda **kw: krlib.attention_paged(**good, **kw),
+                 lambda **kw: krlib.qk_norm_rope_paged(torch.zeros(3, 8 * 64, dtype=q.dtype), c, pos, pos, 4,
+                                                       tab, tab, **kw),
+                 lambda **kw: krlib.kv_commit(c, i32(2, 4), i32(2), i32(2, 3), i32(2), **kw)):
+        with pytest.raises(krlib.KrbError, match="status"):
+            call(status=i32(0))
+        with pytest.raises(krlib.KrbError, match="not on a GPU"):
+            call(status=i32(1))
