@@ -116,7 +116,8 @@ int krb_attention_prefill_bf16(const void *qkv, void *out, int S, int HQ, int HK
  * strides multiples of 8 whose rows do not overlap.  page_size is a power of two from 8 on, head_dim 64
  * or 128.  A sequence's tokens live in the pages of its row of a page table (int32 [B,
  * max_pages], row pitch ldp): position p in page table[p / page_size], slot p % page_size.
- * Entries behind a sequence's last page are never read.  max_pages * page_size <= 2^30.
+ * Entries behind a sequence's last page are never read.  max_pages * page_size <= 2^30.  Index
+ * arrays are aligned to their elements.
  *
  * A bad value that only the device sees (an index outside its range, impossible lengths) is
  * never followed: it sets bit 7 or 8 of *status (may be NULL), and what the call then leaves

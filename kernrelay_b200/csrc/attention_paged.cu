@@ -638,10 +638,9 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   const long width = static_cast<long>(a.HQ) * c.head_dim;
   if (a.ldq < width || a.ldo < width || a.ldq % 8 || a.ldo % 8)
     throw CudaError("attention_paged: row pitch too small or not a multiple of 8");
-  for (const void *p : {a.q, static_cast<const void *>(a.out),
-                        static_cast<const void *>(a.workspace)})
-    if (reinterpret_cast<uintptr_t>(p) % 16)
-      throw CudaError("attention_paged: pointers must be 16-byte aligned");
+  check_aligned({a.q, a.out, a.workspace}, 16, "attention_paged: pointers must be 16-byte aligned");
+  check_aligned({a.page_table, a.kv_lens, a.q_starts, a.mask, a.status}, 4,
+                "attention_paged: table, lengths, starts, mask and status must be 4-byte aligned");
   if (a.max_pages <= 0 || a.ldp < a.max_pages)
     throw CudaError("attention_paged: page table narrower than its rows");
   if (int64_t(a.max_pages) * c.page_size > (int64_t(1) << 30))

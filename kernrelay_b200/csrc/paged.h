@@ -1,6 +1,7 @@
 // The paged K/V cache as the kernels see it, and the launchers of its operators.
 #pragma once
 
+#include <initializer_list>
 #include <utility>
 
 #include "common.h"
@@ -33,6 +34,9 @@ void launch_pdl(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream
 // Throws on a cache the operators do not take (null pointers, sizes, alignment, strides whose
 // rows overlap); `layer` in [0, layers).
 void check_cache(const krb_kv_cache *c, int layer, const char *what);
+
+// Throws unless every address is a multiple of `bytes` (null is one).
+void check_aligned(std::initializer_list<const void *> ps, size_t bytes, const char *why);
 
 // Whether any of n rows of `wa` 2-byte elements at pitch `la` shares an element with any of n rows
 // of `wb` at pitch `lb` (pitches no smaller than their rows).

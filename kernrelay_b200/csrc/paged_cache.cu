@@ -47,6 +47,11 @@ void check_cache(const krb_kv_cache *c, int layer, const char *what) {
   check_strides(c->v_stride, *c, what);
 }
 
+void check_aligned(std::initializer_list<const void *> ps, size_t bytes, const char *why) {
+  for (const void *p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % bytes) throw CudaError(why);
+}
+
 bool rows_overlap(const void *a, long la, long wa, const void *b, long lb, long wb, int n) {
   using i128 = __int128;  // pitches are the caller's
   const i128 a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
@@ -383,11 +388,10 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
   if (max_pos <= 0) throw CudaError("qk_norm_rope_paged: empty rope tables");
   if (ldqkv < static_cast<long>(nh) * D || ldq < static_cast<long>(HQ) * D || ldqkv % 8 || ldq % 8)
     throw CudaError("qk_norm_rope_paged: row pitch too small or not a multiple of 8");
-  for (const void *p : {qkv, static_cast<const void *>(q_out), static_cast<const void *>(cos_tab),
-                        static_cast<const void *>(sin_tab), static_cast<const void *>(q_norm),
-                        static_cast<const void *>(k_norm)})
-    if (reinterpret_cast<uintptr_t>(p) % 16)
-      throw CudaError("qk_norm_rope_paged: pointers must be 16-byte aligned");
+  check_aligned({qkv, q_out, cos_tab, sin_tab, q_norm, k_norm}, 16,
+                "qk_norm_rope_paged: pointers must be 16-byte aligned");
+  check_aligned({positions, slots}, 8, "qk_norm_rope_paged: positions and slots must be 8-byte aligned");
+  check_aligned({status}, 4, "qk_norm_rope_paged: status must be 4-byte aligned");
   if (!(q_out == qkv && (ldq == ldqkv || N == 1)) &&
       rows_overlap(qkv, ldqkv, static_cast<long>(nh) * D, q_out, ldq, static_cast<long>(HQ) * D, N))
     throw CudaError("qk_norm_rope_paged: q_out overlaps qkv, and is not its q columns");
@@ -503,6 +507,7 @@ void kv_commit(const krb_kv_cache &c, const int32_t *page_table, long ldp, int m
   if (!page_table || !bases || !accepted || !counts) throw CudaError("kv_commit: null pointer");
   if (max_pages <= 0 || ldp < max_pages || lda < A)
     throw CudaError("kv_commit: page table or accepted list narrower than its rows");
+  check_aligned({page_table, bases, accepted, counts, status}, 4, "kv_commit: pointers must be 4-byte aligned");
   if ((int64_t(max_pages) << ilog2(c.page_size)) > (int64_t(1) << 30))
     throw CudaError("kv_commit: max_pages * page_size above 2^30");
   CommitArgs a{};

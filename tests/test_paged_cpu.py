@@ -388,3 +388,29 @@ def test_masks_and_status_without_elements(krlib):
             call(status=i32(0))
         with pytest.raises(krlib.KrbError, match="not on a GPU"):
             call(status=i32(1))
+
+
+def test_index_arrays_between_their_elements(krlib):
+    """Addresses that an index array cannot have: refused, where the kernels would fault on them."""
+    L, d = krlib.lib(), ctypes.addressof(keep := _desc(krlib))
+    base = 1 << 30
+
+    def append(pos=64, slots=64, status=None):
+        return L.krb_qk_norm_rope_paged(d, 0, base, W3, 16, W, pos, slots, 3, 28, 16, 16, 8, None, None, 1e-6,
+                                        status, None)
+
+    def attention(table=64, lens=64, starts=64, mask=None, status=None):
+        return L.krb_attention_paged(d, 0, base, W, 16, W, 3, 28, table, 8, 8, lens, starts, 2, 1, mask, 1, 1,
+                                     0.1, None, 0, status, None)
+
+    def commit(table=64, bases=64, acc=64, counts=64, status=None):
+        return L.krb_kv_commit(d, table, 8, 8, bases, acc, 4, 4, counts, 2, status, None)
+
+    for call, size, names in ((append, 8, ("pos", "slots")), (append, 4, ("status",)),
+                              (attention, 4, ("table", "lens", "starts", "mask", "status")),
+                              (commit, 4, ("table", "bases", "acc", "counts", "status"))):
+        for name in names:
+            for off in (1, 2, size - 1, size // 2):
+                assert call(**{name: 64 + off}) == 1, name
+                assert f"{size}-byte aligned" in _message(krlib), name
+    del keep
