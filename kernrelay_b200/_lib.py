@@ -338,6 +338,8 @@ class KVCache:
         n = self._workspaces.get((HQ, max_q))
         if n is None:
             import torch
+            if not 0 <= max_q < 2 ** 31:  # a C int would take it modulo 2^32
+                raise KrbError(f"attention_paged: bad max_q {max_q}")
             if self.index < 0:
                 raise KrbError("KVCache: the cache is not on a GPU")
             with torch.cuda.device(self.index):
@@ -360,6 +362,11 @@ def _refuse(what, name, t, dtype, dim):
     raise KrbError(f"{what}: {name} must be a {dim}-d {dtype} tensor on the cache's device with its "
                    f"last axis contiguous, got {t.dim()}-d {t.dtype} on {t.device}, strides "
                    f"{tuple(t.stride())}")
+
+
+def _check_layer(what, cache, layer):
+    if not 0 <= layer < cache.layers:
+        raise KrbError(f"{what}: no such layer ({layer} of {cache.layers})")
 
 
 def _enter(cache):
@@ -390,6 +397,7 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
         _refuse(what, "cos", cos, bf, 2)
     if not _is(sin, bf, index, 2):
         _refuse(what, "sin", sin, bf, 2)
+    _check_layer(what, cache, layer)
     D = cache.head_dim
     N, width = qkv.shape
     if width != (HQ + 2 * cache.heads) * D:
@@ -441,6 +449,7 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
         _refuse(what, "kv_lens", kv_lens, i32, 1)
     if not _is(q_starts, i32, index, 1):
         _refuse(what, "q_starts", q_starts, i32, 1)
+    _check_layer(what, cache, layer)
     N, width = q.shape
     HQ = width // cache.head_dim
     if HQ * cache.head_dim != width:

@@ -414,3 +414,24 @@ def test_index_arrays_between_their_elements(krlib):
                 assert call(**{name: 64 + off}) == 1, name
                 assert f"{size}-byte aligned" in _message(krlib), name
     del keep
+
+
+@pytest.mark.parametrize("layer", [-1, 2, 2 ** 32, 2 ** 32 + 1, -2 ** 32])
+def test_layers_outside_the_cache(krlib, layer):
+    """Refused as they are, not modulo 2^32."""
+    import torch
+    c = _cpu_cache(krlib)
+    c._workspaces[4, 1] = 64
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    q, pos = torch.zeros(3, 4 * 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    tab = torch.zeros(9, 64, dtype=torch.bfloat16)
+    with pytest.raises(krlib.KrbError, match="no such layer"):
+        krlib.attention_paged(q, c, i32(2, 4), i32(2), i32(3), 1, 0.1, layer=layer)
+    with pytest.raises(krlib.KrbError, match="no such layer"):
+        krlib.qk_norm_rope_paged(torch.zeros(3, 8 * 64, dtype=q.dtype), c, pos, pos, 4, tab, tab, layer=layer)
+
+
+@pytest.mark.parametrize("max_q", [-1, 2 ** 31, 2 ** 32 + 1, 2 ** 32])
+def test_max_q_outside_an_int(krlib, max_q):
+    with pytest.raises(krlib.KrbError, match="max_q"):
+        _cpu_cache(krlib).attention_workspace(4, max_q)
