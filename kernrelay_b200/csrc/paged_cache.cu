@@ -92,7 +92,6 @@ struct AppendArgs {
   int N, HQ, HKV, max_pos, page_shift;
   int64_t total_slots;
   float eps;
-  bool stream_out;
   uint32_t *status;
 };
 
@@ -138,7 +137,11 @@ __device__ __forceinline__ uint4 ldg4(const void *p) {
 // tokens of 32 + 2 x 8 heads of 128 with norms, 203 MB, 38.1 us, 0.83 of the copy's rate (rows
 // through L1 42.7; unpaired and 32 / 40 / 48 warps 48.8 / 44.2 / 45.6); 2400 of them 10.8 us, 0.87.
 // Tried: several heads per warp with the table products in registers (54 us), whole rows by bulk copies
-// into shared memory (42.2 us, and twice the time at 14 + 2 x 2 heads of 64).
+// into shared memory (42.2 us, and twice the time at 14 + 2 x 2 heads of 64), stores that leave L2 first
+// (up to 2 us less by itself, nothing between a producer of the rows and the attention that reads the
+// output: 8 prompts of 32 + 2 x 8 heads, 101 / 201 / 302 MB of output, the three together with plain stores
+// 208.6 / 515 / 1004 us, with those 208.4 / 514 / 998; 32 prompts 147.6 / 308.7 / 496 and 146.5 / 308.8 /
+// 498; append and attention alone 175.8 / 434 / 906 and 178.2 / 434 / 901).
 template <int D, bool F16>
 __global__ void __launch_bounds__(128, 10) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
@@ -159,10 +162,7 @@ __global__ void __launch_bounds__(128, 10) append_kernel(const AppendArgs a) {
   const bool pos_ok = pos >= 0 && pos < a.max_pos;
   if (!pos_ok && h == 0 && j == 0) report_status(a.status, kStatusBadIndex);
 
-  auto store = [&](uint16_t *to, const uint4 &w) {
-    if (a.stream_out) __stcs(reinterpret_cast<uint4 *>(to), w);
-    else *reinterpret_cast<uint4 *>(to) = w;
-  };
+  auto store = [&](uint16_t *to, const uint4 &w) { *reinterpret_cast<uint4 *>(to) = w; };
   uint16_t *dst;
   if (h < a.HQ) {
     dst = a.q_out + n * a.ldq + h * D + j;
@@ -422,10 +422,6 @@ void qk_norm_rope_paged(const krb_kv_cache &c, int layer, const void *qkv, long 
   a.total_slots = int64_t(c.pages) * c.page_size;
   a.eps = eps;
   a.status = status;
-  // Output that the next kernel would not find in L2 (126 MB) as a whole goes past it: 42.1 -> 38.1 us
-  // for 101 MB (8192 tokens of 32 + 2 x 8 heads of 128); at 50 MB it would gain a twentieth and cost
-  // the reader.
-  a.stream_out = static_cast<int64_t>(N) * nh * D * 2 > (int64_t(64) << 20);
   if (D == 128 && c.dtype) launch_append<128, true>(a, stream);
   else if (D == 128) launch_append<128, false>(a, stream);
   else if (c.dtype) launch_append<64, true>(a, stream);
