@@ -120,7 +120,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int box = 1 << box_shift;
     const uint32_t box_bytes = box * 128;
     PageFeed feed;
-    const uint64_t policy = p.kv_once ? l2_policy_evict_first() : l2_policy_evict_normal();
+    // The keys are first to leave L2.  Without / with: 64 decoding sequences 108.1 / 104.6 us, two long
+    // ones 77.5 / 76.1, 64 sequences that share 2000, 8000 or 32000 positions 99.9 / 98.2, 114.1 / 112.0
+    // and 390.6 / 381.4, 16 of 4000 (131 MB) 30.1 / 28.0; caches that stay in L2 between calls, alone or
+    // beside 30 to 120 MB of other reads, take the same or less.
+    const uint64_t policy = l2_policy_evict_first();
     int n = 0;  // blocks issued
     bool ok = true;
     while (w.pos < w.end && ok) {
@@ -682,11 +686,6 @@ void attention_paged(const krb_kv_cache &c, int layer, const PagedAttnArgs &a, c
   p.tpt = pl.tpt;
   p.tile_tok = pl.tile_tok;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  // One unit reads a sequence's keys of a head, and a layer's cache does not stay in L2 (126 MB) from
-  // call to call: 64 decoding sequences 108.1 -> 104.6 us, 2 long ones 77.5 -> 76.1; with the first 32
-  // pages shared by all sequences still 100.2 -> 96.8 (wide trees, whose units share keys, gained nothing).
-  p.kv_once = a.max_q <= pl.tpt &&
-              4.0 * c.pages * c.page_size * c.heads * c.head_dim > double(int64_t(126) << 20);
   p.status = a.status;
   carve_workspace(p, pl.ctas, a.workspace);
 

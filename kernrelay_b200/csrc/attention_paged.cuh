@@ -29,7 +29,6 @@ struct Params {
   int tpt;       // tokens of a unit
   int tile_tok;  // tokens of one 128-row tile of the unit (tcgen05; tpt is one or two tiles)
   int rows;      // rows of a partial result's slot
-  bool kv_once;  // no key is read twice while it could stay in L2: first to leave it
   float scale_log2;
   uint32_t *status;
   // workspace: G descriptors, then per CTA and slot: m and l [rows] (log2 units), O [rows][D]
