@@ -963,3 +963,216 @@ def test_attention_without_tokens(cuda, krlib, max_q):
     torch.cuda.synchronize()
     assert (got == 5.0).all()  # rows of no sequence
     assert cache.attention_workspace(8, 0) == cache.attention_workspace(8, 1) > 0
+
+
+# ---------------------------------------------------------------- refusals in every kernel
+# 28 heads over 4: rows of 1 token are 7 (mma.sync), of 8 tokens 56 (tcgen05, one tile), of 40 two tiles
+TOKENS = [1, 8, 40]
+
+
+def _left(b, out, refused):
+    """Rows of refused sequences, and rows of none, are as they were."""
+    for i in refused:
+        assert (out[b.starts_host[i]:b.starts_host[i + 1]] == 5.0).all(), i
+    assert (out[b.starts_host[-1]:] == 5.0).all()
+
+
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("masked", [False, True])
+def test_refused_lengths_leave_rows(cuda, krlib, T, masked):
+    import torch
+    seqs = [(100, T), (64, T), (10, max(1, T - 1)), (300, T), (0, T)]
+    b = Batch(seqs, 28, 4, 128, 16, seed=T, masked=masked)
+    for lens, bad in (({1: T - 1}, {1}), ({0: -5}, {0}), ({3: 10 ** 9}, {3}), ({4: 0, 2: 2 ** 31 - 1}, {2, 4}),
+                      ({0: -2 ** 31, 1: -1, 2: 0, 3: 0, 4: -1}, {0, 1, 2, 3, 4})):
+        saved = b.lens.clone()
+        for i, n in lens.items():
+            b.lens[i] = n
+        out = b.run(krlib)
+        torch.cuda.synchronize()
+        assert b.status.item() == 1 << 7
+        b.lens.copy_(saved)
+        _left(b, out, bad)
+        b.check(out, only=set(range(5)) - bad)
+    if T > 1:  # more new tokens than max_q
+        out = b.run(krlib, max_q=T - 1)
+        torch.cuda.synchronize()
+        assert b.status.item() == 1 << 7
+        _left(b, out, {0, 1, 3, 4})
+        b.check(out, only={2})
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_refused_starts_leave_rows(cuda, krlib, T):
+    import torch
+    seqs = [(100, T), (64, T), (10, T), (300, T), (0, T)]
+    b = Batch(seqs, 28, 4, 128, 16, seed=T)
+    want = b.run(krlib).clone()
+    for i, x, bad in ((5, b.N + 1, {4}), (0, -1, {0}), (2, b.N + 7, {1, 2}), (3, 2 * T - 1, {2, 3}),
+                      (5, -2 ** 31, {4}), (1, 2 ** 31 - 1, {0, 1})):
+        saved = b.starts.clone()
+        b.starts[i] = x
+        out = b.run(krlib)
+        torch.cuda.synchronize()
+        assert b.status.item() == 1 << 7
+        b.starts.copy_(saved)
+        _left(b, out, bad)
+        for j in set(range(5)) - bad:
+            rows = slice(T * j, T * j + T)
+            b.check(out, only={j})
+            assert torch.isfinite(out[rows]).all()
+    assert torch.equal(b.run(krlib), want)
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_bad_pages_read_as_page_0(cuda, krlib, T):
+    import torch
+    b = Batch([(200, T), (100, T)], 28, 4, 128, 16, seed=2)
+    saved = b.table.clone()
+    b.table[0, 3] = 0
+    want = b.run(krlib).clone()
+    for bad in (b.pages, -1, 2 ** 31 - 1, -2 ** 31):
+        b.table[0, 3] = bad
+        out = b.run(krlib)
+        torch.cuda.synchronize()
+        assert b.status.item() == 1 << 8
+        b.check(out, only={1})
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+        _left(b, out, set())
+    b.table.copy_(saved)
+    out = b.run(krlib)
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    b.check(out)
+
+
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("heads,B", [(8, 2), (4, 33)])
+def test_refused_calls(cuda, krlib, T, heads, B):
+    """More than 2^26 blocks of 64 keys in a sequence, or 2^31 in the batch: the whole call is refused
+    before a key is read (2^30 positions are 2^24 blocks a head)."""
+    import torch
+    page, D = 1024, 64
+    k, v = _cache_tensors(1, 2, heads, page, D, torch.bfloat16, "hnd", fill=1.0)
+    table = torch.zeros(B, 2 ** 30 // page, dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), 2 ** 30, dtype=torch.int32, device="cuda")
+    if heads == 8:
+        lens[0] = 100
+    starts = torch.arange(B + 1, dtype=torch.int32, device="cuda") * T
+    q = torch.ones(B * T, heads * D, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 5.0)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    krlib.attention_paged(q, krlib.KVCache(k, v), table, lens, starts, T, 0.1, out=out, status=status)
+    torch.cuda.synchronize()
+    assert status.item() == 1 << 7
+    assert (out == 5.0).all()
+    lens.fill_(T + 100)  # the same arrays, lengths that are taken
+    status.zero_()
+    krlib.attention_paged(q, krlib.KVCache(k, v), table, lens, starts, T, 0.1, out=out, status=status)
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    assert (out == 1.0).all()
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_graph_follows_lengths_and_starts(cuda, krlib, T):
+    import torch
+    seqs = [(900, T), (333, T), (64, T)]
+    b = Batch(seqs, 28, 4, 128, 16, seed=9)
+    b.run(krlib)
+    out = torch.full((b.N, b.HQ * b.D), 5.0, dtype=b.dt, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache = krlib.KVCache(b.k, b.v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        krlib.attention_paged(b.q, cache, b.table, b.lens, b.starts, T, b.scale, out=out, status=status)
+    for cut, new in ((0, (T, T, T)), (17, (T, 0, T)), (63, (max(1, T - 3), T, 1)), (5, (0, 0, 0)),
+                     (1, (T, T, T))):
+        lens = [c - cut + t for (c, _), t in zip(seqs, new)]
+        starts = [sum(new[:i]) for i in range(4)]
+        b.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        b.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        now = Batch(seqs, 28, 4, 128, 16, seed=9)
+        now.seqs, now.starts_host = [(c - cut, t) for (c, _), t in zip(seqs, new)], starts
+        now.sees = [torch.ones(t, t, dtype=torch.bool, device="cuda").tril() for t in new]
+        now.K, now.V = ([x[:n] for x, n in zip(xs, lens)] for xs in (now.K, now.V))
+        now.check(out)
+        assert (out[starts[-1]:] == 5.0).all()
+
+
+@pytest.mark.parametrize("T", [8, 40])
+@pytest.mark.parametrize("masked", [False, True])
+def test_same_result_twice_many_rows(cuda, krlib, T, masked):
+    import torch
+    b = Batch([(5000, T), (77, T), (2500, T)], 28, 4, 128, 16, seed=4, masked=masked)
+    a = b.run(krlib)
+    for _ in range(5):
+        assert torch.equal(a, b.run(krlib))
+
+
+@pytest.mark.parametrize("B,n", [(1, 63), (1, 64), (3, 65), (1, 1999), (70, 1999), (1, 8191), (50, 4097)])
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("HQ,HKV,D,dtype", [(28, 4, 128, "bf16"), (14, 2, 64, "fp16")])
+def test_every_key_counts_once(cuda, krlib, B, n, T, HQ, HKV, D, dtype):
+    """Scores of 0, and values of one in column j % D for key j: a column is its number of keys over n, so
+    one key lost or taken twice moves it by D / n, far more than the roundings (of 1 / n, of the product
+    and the output's: the sums are whole numbers)."""
+    import torch
+    dt, page, g = _dt(dtype), 16, _gen(n)
+    need = -(-n // page)
+    v = torch.eye(D, device="cuda")[torch.arange(need * page, device="cuda") % D].to(dt)
+    v = v.view(1, need, page, 1, D).expand(1, need, page, HKV, D).transpose(2, 3).contiguous()
+    k = torch.randn(v.shape, generator=g, device="cuda").to(dt)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(need, dtype=torch.int32, device="cuda").repeat(B, 1)
+    mask = torch.full((B * T, 2), -1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(B * T, HQ * D, dtype=dt, device="cuda")
+    out = krlib.attention_paged(q, krlib.KVCache(k, v), table, i32([n] * B),
+                                i32([T * i for i in range(B + 1)]), T, 0.1, mask=mask)
+    torch.cuda.synchronize()
+    count = torch.bincount(torch.arange(n, device="cuda") % D, minlength=D).double()
+    ref = count / n
+    bound = (torch.finfo(dt).eps / 2 + 2.0 ** -22) * ref + 2.0 ** -25 * (dt == torch.float16)
+    assert D / n > 2 * bound.max() / ref.max() or n < D
+    assert ((out.double().view(B * T, HQ, D) - ref).abs() <= bound).all()
+
+
+# ---------------------------------------------------------------- streams
+def test_stream_argument(cuda, krlib):
+    """append, page copies and commits on the stream that they are given, behind its work and not behind
+    (or in) the current one's."""
+    import torch
+    HQ, HKV, D, page, n = 8, 2, 128, 16, 256
+    g, dt = _gen(1), torch.bfloat16
+    cos, sin = _rope_tables(n, D)
+    pos = torch.arange(n, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, bases, accepted, counts = i32([list(range(n // page))]), i32([100]), i32([[1, 5, 9]]), i32([3])
+    busy = torch.randn(4096, 4096, generator=g, device="cuda")
+    x = torch.randn(n, (HQ + 2 * HKV) * D, generator=g, device="cuda").to(dt)
+
+    def step(**kw):
+        k, v = _cache_tensors(1, n // page + 1, HKV, page, D, dt, "hnd", fill=0.0)
+        cache, src = krlib.KVCache(k, v), torch.zeros_like(x)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(kw.get("stream") or torch.cuda.current_stream()):
+            for _ in range(3):
+                (busy @ busy).sum()
+            src.copy_(x)
+        q = krlib.qk_norm_rope_paged(src, cache, pos, pos, HQ, cos, sin, status=status, **kw)
+        krlib.kv_copy_pages(cache, [3], [n // page], **kw)
+        krlib.kv_commit(cache, table, bases, accepted, counts, status=status, **kw)
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        return q, k, v
+
+    want, got = step(), step(stream=torch.cuda.Stream())
+    for a, b in zip(want, got):
+        assert torch.equal(a, b) and a.abs().max() > 0
+    assert torch.equal(want[1][0, n // page], want[1][0, 3])
