@@ -1176,3 +1176,70 @@ def test_stream_argument(cuda, krlib):
     for a, b in zip(want, got):
         assert torch.equal(a, b) and a.abs().max() > 0
     assert torch.equal(want[1][0, n // page], want[1][0, 3])
+
+
+# ---------------------------------------------------------------- a whole step captured
+@pytest.mark.parametrize("T", TOKENS)
+def test_step_captured(cuda, krlib, T):
+    """Append, attention, page copy and commit in one graph: a replay on new rows, slots, lengths, masks
+    and lists does what the calls do."""
+    import torch
+    HQ, HKV, D, page, B, L = 28, 4, 128, 16, 3, 2
+    dt, g, need = torch.bfloat16, _gen(T), 12
+    pages = B * need + 1
+    cos, sin = _rope_tables(need * page, D)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    words = -(-T // 32)
+
+    def inputs(seed):
+        r = random.Random(seed)
+        ids = list(range(pages - 1))
+        r.shuffle(ids)
+        rows = [ids[b * need:(b + 1) * need] for b in range(B)]
+        ctx = [r.randint(0, need * page - T) for _ in range(B)]
+        at = [(b, c + t) for b, c in enumerate(ctx) for t in range(T)]
+        acc = [sorted(r.sample(range(T), min(T, 2))) + [-1] * (2 - min(T, 2)) for _ in range(B)]
+        masks = torch.cat([_tree(r, T, words)[0] for _ in range(B)])
+        return dict(qkv=torch.randn(B * T, (HQ + 2 * HKV) * D, generator=_gen(seed), device="cuda").to(dt),
+                    pos=torch.tensor([p for _, p in at], device="cuda"),
+                    slots=torch.tensor([rows[b][p // page] * page + p % page for b, p in at], device="cuda"),
+                    table=i32(rows), lens=i32([c + T for c in ctx]), bases=i32(ctx), acc=i32(acc),
+                    counts=i32([r.randint(0, min(T, 2)) for _ in range(B)]), mask=masks.cuda())
+
+    starts = i32([T * i for i in range(B + 1)])
+    k0, v0 = _cache_tensors(L, pages, HKV, page, D, dt, "nhd", g=g)
+
+    def step(s, cache, status):
+        outs = []
+        for layer in range(L):
+            q = krlib.qk_norm_rope_paged(s["qkv"], cache, s["pos"], s["slots"], HQ, cos, sin, layer=layer,
+                                         status=status)
+            outs.append(krlib.attention_paged(q, cache, s["table"], s["lens"], starts, T, D ** -0.5,
+                                              mask=s["mask"], layer=layer, status=status))
+        krlib.kv_copy_pages(cache, [3], [pages - 1])
+        krlib.kv_commit(cache, s["table"], s["bases"], s["acc"], s["counts"], status=status)
+        return outs
+
+    held, status = inputs(0), torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = k0.clone(), v0.clone()
+    cache = krlib.KVCache(k, v)
+    step(held, cache, status)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(held, cache, status)
+    for seed in (1, 2, 3):
+        new = inputs(seed)
+        for name, x in new.items():
+            held[name].copy_(x)
+        k.copy_(k0)
+        v.copy_(v0)
+        graph.replay()
+        torch.cuda.synchronize()
+        k1, v1 = k0.clone(), v0.clone()
+        want = step(new, krlib.KVCache(k1, v1), status)
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert torch.equal(k, k1) and torch.equal(v, v1)
+        assert not torch.equal(outs[0], outs[1]) and not torch.equal(k, k0)
