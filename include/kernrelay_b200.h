@@ -120,8 +120,9 @@ int krb_attention_prefill_bf16(const void *qkv, void *out, int S, int HQ, int HK
  * arrays are aligned to their elements.
  *
  * A bad value that only the device sees (an index outside its range, impossible lengths) is
- * never followed: it sets bit 7 or 8 of *status (may be NULL), and what the call then leaves
- * out is stated per call. */
+ * never followed: it sets bit 7 or 8 of *status (may be NULL: then nothing tells of it), and what the
+ * call then leaves out is stated per call.  Bits 0 to 2 (attention): a wait inside a kernel ran out
+ * after 2 s, and the output is incomplete. */
 typedef struct krb_kv_cache {
   void *k, *v;
   int dtype; /* 0: bf16, 1: fp16 */
@@ -161,6 +162,9 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * (So does, for the whole call, a sequence of more than 2^26 blocks of 64 keys, its row tiles and
  * KV heads counted each, or 2^31 in all.)
  * A page outside [0, pages) sets bit 8 and is read as page 0.
+ * Scores, softmax statistics and sums are fp32; a probability is rounded to the cache dtype before it
+ * meets its value (to 2^-9 of itself in bf16, 2^-12 in fp16, there no finer than 2^-32 of the row's
+ * largest), the output once more at the store.
  * out may not overlap q (refused).
  * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call
  * alone until it is done; calls in order on one stream may share one. */
@@ -186,7 +190,7 @@ int krb_kv_copy_pages(const krb_kv_cache *cache, const int32_t *src, const int32
  * (accepted int32 [B, A], row pitch lda; device arrays).  accepted[b] must ascend strictly from
  * >= 0, so a row is never overwritten before it is read.  A sequence whose counts, bases,
  * accepted or pages are out of range or order sets bit 8 and is left as it was.  The pages that
- * two sequences move rows in must differ. */
+ * a sequence moves rows in must differ from each other and from those of other sequences. */
 int krb_kv_commit(const krb_kv_cache *cache, const int32_t *page_table, int64_t ldp, int max_pages,
                   const int32_t *bases, const int32_t *accepted, int64_t lda, int A,
                   const int32_t *counts, int B, uint32_t *status, void *stream);

@@ -311,7 +311,11 @@ class KVCache:
     page_size, head_dim], or [layers, pages, ...], bf16 or fp16, head_dim contiguous, the other
     axes of any strides (pass `x.transpose(-3, -2)` where the slot axis is stored outside the
     heads').  page_size: a power of two from 8 on; head_dim 64 or 128.  The handle keeps the
-    tensors; make it once per cache."""
+    tensors; make it once per cache.
+
+    The operators below run on the current stream of the cache's device, or on stream=.  Outputs and
+    workspaces that a call allocates belong to that stream; that its inputs are ready on it, and live
+    until it is done with them (torch's record_stream), is the caller's, as in torch."""
 
     def __init__(self, k, v):
         import torch
@@ -384,7 +388,8 @@ def qk_norm_rope_paged(qkv, cache, positions, slots, HQ, cos, sin, q_norm=None, 
     """Per-head norms (optional) and RoPE at positions[n] for the q and k heads of
     qkv [N, (HQ+2*HKV)*D]; returns the rotated q [N, HQ*D] and writes the k and v heads to slot
     slots[n] = page * page_size + offset of the cache's `layer` (-1: not written).  positions and
-    slots int64 [N]; cos / sin bf16 [max_pos, D]."""
+    slots int64 [N]; cos / sin bf16 [max_pos, D].  out may be the q columns of qkv and may not overlap it
+    otherwise."""
     import torch
     what, dt, index, i64, bf = "qk_norm_rope_paged", cache.dtype, cache.index, torch.int64, torch.bfloat16
     if not _is(qkv, dt, index, 2):
@@ -437,8 +442,10 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
     of the new ones, those up to itself (mask None) or those of its mask bits (int32 [N, words],
     bit j % 32 of word j / 32 for new token j; a tree of drafted tokens).  page_table int32
     [B, max_pages], kv_lens int32 [B], q_starts int32 [B+1], all on the device; max_q: no less
-    than any T_b.  workspace: a uint8 tensor of cache.attention_workspace(HQ, max_q) bytes that no
-    other call uses until this one is done (default: allocated per call)."""
+    than any T_b.  out may not overlap q.  Rows that belong to no sequence, and those of a sequence that
+    the device refuses (status), are not written: in the default out, a fresh tensor, they hold
+    whatever its memory held.  workspace: a uint8 tensor of cache.attention_workspace(HQ, max_q) bytes
+    that no other call uses until this one is done (default: allocated per call).  stream: see KVCache."""
     import torch
     what, dt, index, i32 = "attention_paged", cache.dtype, cache.index, torch.int32
     if not _is(q, dt, index, 2):
@@ -494,8 +501,8 @@ def attention_paged(q, cache, page_table, kv_lens, q_starts, max_q, scale, mask=
 
 def kv_copy_pages(cache, src, dst, stream=None):
     """Copy page src[i] to page dst[i], K and V of all layers (a fork's page of its own, or pages
-    moved together).  src, dst: host sequences of page numbers; no page is written twice, or both
-    read and written."""
+    moved together).  src, dst: host sequences of page numbers (bytes, too, element by element); no
+    page is written twice, or both read and written."""
     what, n = "kv_copy_pages", len(src)
     if len(dst) != n:
         raise KrbError(f"{what}: src and dst differ in length")

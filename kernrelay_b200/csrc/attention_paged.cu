@@ -7,8 +7,9 @@
 // at the memory, which then serves the SMs less evenly: 110.6 us against 108.3 in the first case
 // below), the rows of all query heads that share a KV head go through the tensor cores together, and
 // the four warps of a CTA split the keys, so that a block costs each a quarter.
-// Measured: 64 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads of 128,
-// 104.6 us, 98 % of what 659 MB take at the copy's rate; 2 sequences of 98 and 131 thousand, 76 us, 95 %.
+// Measured (calls in a graph, three sets of inputs in turn): 64 sequences of 2 to 8 thousand positions,
+// 28 query heads over 4 KV heads of 128, 106 us, 97 % of the copy's rate for 659 MB; 2 sequences of 98 and
+// 131 thousand, 77 us, 94 %.  One call after the other through the Python wrapper: 109 and 78.6 us.
 #include <algorithm>
 #include <string>
 

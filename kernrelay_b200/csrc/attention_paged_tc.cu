@@ -14,11 +14,14 @@
 // clock are there), MUFU 2100; measured are 4000, since a wait on an mbarrier keeps an issuer from
 // feeding the pipe for some 115 clocks even when it has come (its queue holds one or two products).
 // A piece's start and end (first scores, last product, O out) cost some 5000 more.
-// Measured: 64-token trees (8 sequences of 2 to 8 thousand positions, 28 query heads over 4 KV heads
-// of 128) 62 us, 0.32 of their flop at the library's rate; two chunks of 1024 tokens over 1 and
-// 8 thousand positions 187 us, 0.44; 8-token trees (32 rows, 169 MB) 37 us, 0.70 of the copy's rate,
-// 64 sequences of them 117 us, 0.89.  With one tile a ring of 8 blocks is as good as 12 or better (38.1 us
-// against 39.1, without the L2 hint): a deeper queue serves the SMs less evenly.
+// Measured (calls in a graph, three sets of inputs in turn): 64-token trees (8 sequences of 2 to 8
+// thousand positions, 28 query heads over 4 KV heads of 128) 62 to 64 us, 0.32 of their flop at the
+// library's rate; two chunks of 1024 tokens over 1 and 8 thousand positions 189 to 200 us, 0.41 to 0.44;
+// 8-token trees (32 rows, 169 MB) 38 us, 0.69 of the copy's rate, 64 sequences of them 122 us, 0.84.
+// The ring's depth hardly matters: 8-token trees at head_dim 128 take 37.9 us with 8 blocks, 38.0 with
+// 10, and without the L2 hint 38.1 with 8, 39.1 with 12 (a deeper queue serves the SMs less evenly);
+// wide trees 62.5 with 10, 61.7 with 8, chunks 197 and 196; head_dim 64 (14 heads over 2), 8 / 16 / 24
+// blocks: 23.9 / 24.0 / 24.2, wide trees 54.4 / 54.5 / 54.9, chunks 156.7 / 156.9 / 156.1.
 // Tried, the trees' and the chunks' time: 128-key blocks with one S stage (70, 205: the chain softmax
 // -> PV -> QK), these with half blocks of P (69, 201) and an issuer per tile (79, 215); one issuer for
 // all products on two stages (83, 239); QK issuers per tile on two stages (69, 203).

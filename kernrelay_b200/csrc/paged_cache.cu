@@ -133,15 +133,16 @@ __device__ __forceinline__ uint4 ldg4(const void *p) {
 //
 // Bound: HBM at size (every value read and written once), a launch when small.  What it takes is
 // loads in flight, and that is warps: the halves are rotated one after the other, in paired fp32, so
-// that forty warps are resident, and the rows, read once, leave L1 to the tables.  Measured: 8192
-// tokens of 32 + 2 x 8 heads of 128 with norms, 203 MB, 38.1 us, 0.83 of the copy's rate (rows
-// through L1 42.7; unpaired and 32 / 40 / 48 warps 48.8 / 44.2 / 45.6); 2400 of them 10.8 us, 0.87.
+// that forty warps are resident, and the rows, read once, leave L1 to the tables.  Measured (calls in a
+// graph, three sets of inputs in turn): 8192 tokens of 32 + 2 x 8 heads of 128 with norms, 203 MB, 42 us,
+// 0.75 of the copy's rate (rows through L1 the same); 2400 of them 11.3 us, 0.83 (13.6).  Before rows went
+// past L1: unpaired, with 32 / 40 / 48 warps, 48.8 / 44.2 / 45.6 us, paired 43.
 // Tried: several heads per warp with the table products in registers (54 us), whole rows by bulk copies
 // into shared memory (42.2 us, and twice the time at 14 + 2 x 2 heads of 64), stores that leave L2 first
-// (up to 2 us less by itself, nothing between a producer of the rows and the attention that reads the
-// output: 8 prompts of 32 + 2 x 8 heads, 101 / 201 / 302 MB of output, the three together with plain stores
-// 208.6 / 515 / 1004 us, with those 208.4 / 514 / 998; 32 prompts 147.6 / 308.7 / 496 and 146.5 / 308.8 /
-// 498; append and attention alone 175.8 / 434 / 906 and 178.2 / 434 / 901).
+// (__stcs: 39.5 us by itself, 11.9 for 2400 tokens, but the attention behind it pays: append and
+// attention of 8 prompts, 101 / 201 MB of output, 175.0 / 468 us with plain stores, 176.4 / 472 with
+// those; between a QKV and an output GEMM of a layer 727.5 / 1577 and 729 / 1577, 32 prompts 659.7 /
+// 1357.6 and 659.5 / 1360).
 template <int D, bool F16>
 __global__ void __launch_bounds__(128, 10) append_kernel(const AppendArgs a) {
   constexpr int HALF = D / 2;
