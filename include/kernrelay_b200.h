@@ -159,11 +159,12 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * HQ / HKV <= 64, scale > 0.  T_b = 0 is allowed.
  * A sequence with T_b > max_q, kv_lens[b] < T_b or > max_pages * page_size, or rows outside
  * [0, N) sets bit 7 and its rows are left as they were, like rows that belong to no sequence.
+ * (Where starts fall, two sequences that are taken may name one row: it holds either's result.)
  * (So does, for the whole call, a sequence of more than 2^26 blocks of 64 keys, its row tiles and
  * KV heads counted each, or 2^31 in all.)
  * A page outside [0, pages) sets bit 8 and is read as page 0.
  * Scores, softmax statistics and sums are fp32; a probability is rounded to the cache dtype before it
- * meets its value (to 2^-9 of itself in bf16, 2^-12 in fp16, there no finer than 2^-32 of the row's
+ * meets its value (to 2^-8 of itself in bf16, 2^-11 in fp16, there no finer than 2^-32 of the row's
  * largest), the output once more at the store.
  * out may not overlap q (refused).
  * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call

@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             o[d][3] *= alpha[1];
           }
         }
-        // P enters the second product in the cache's type, rounded by up to 2^-9 (bf16) or 2^-12
+        // P enters the second product in the cache's type, rounded by up to 2^-8 (bf16) or 2^-11
         // (fp16) of itself; a row's largest is a power of two, so exact.  The row sum takes the
         // fp32 values.
         uint32_t pf[NT / 2][4];

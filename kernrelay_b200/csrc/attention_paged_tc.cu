@@ -135,7 +135,7 @@ __device__ __forceinline__ float exp_block(const uint32_t (&s)[2][32], float sca
     const uint64_t x = pack_f32x2(s[e >> 4][(2 * e) & 31], s[e >> 4][(2 * e + 1) & 31]);
     const float2 a = unpack_f32x2(fma_f32x2(x, sc, mo));
     const float p0 = exp2_mufu(a.x), p1 = exp2_mufu(a.y);
-    // P in the cache's type, rounded by up to 2^-9 (bf16) or 2^-12 (fp16) of itself, the largest one
+    // P in the cache's type, rounded by up to 2^-8 (bf16) or 2^-11 (fp16) of itself, the largest one
     // too where the offset lags; the row sum takes the fp32 values (the rounded ones gave the same
     // error for a tenth more time)
     pk[e] = pack2<F16>(p0, p1);
