@@ -165,7 +165,8 @@ int krb_qk_norm_rope_paged(const krb_kv_cache *cache, int layer, const void *qkv
  * A page outside [0, pages) sets bit 8 and is read as page 0.
  * Scores, softmax statistics and sums are fp32; a probability is rounded to the cache dtype before it
  * meets its value (to 2^-8 of itself in bf16, 2^-11 in fp16, there no finer than 2^-32 of the row's
- * largest), the output once more at the store.
+ * largest), the output once more at the store.  Scores scale * q.k are to stay below 9e7 in magnitude (2^27
+ * over log2(e); fp32 holds them to 8 there).
  * out may not overlap q (refused).
  * workspace: krb_attention_paged_workspace bytes (16-byte aligned, any content), of this call
  * alone until it is done; calls in order on one stream may share one. */

@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int x = 0; x < 2; ++x) {
           top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
           top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-          m[x] = fmaxf(m[x], top[x] * p.scale_log2);
+          m[x] = fmaxf(m[x], row_max(top[x], p.scale_log2));
           // a row that has seen nothing yet has no maximum: any offset gives its zeros
           off[x] = m[x] == -INFINITY ? 0.f : m[x];
           alpha[x] = exp2_mufu(mx[x] - off[x]);
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         // fp32 values.
         uint32_t pf[NT / 2][4];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) off[x] -= p_shift<F16, 0>();
+        for (int x = 0; x < 2; ++x) off[x] = p_offset<F16, 0>(m[x]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll

@@ -294,10 +294,18 @@ __device__ __forceinline__ float *slot_o(const Params &p, int cta, int slot) {
 // one, so P uses the type up to 2^15 (m and the sums of all pieces carry the same factor, which the
 // division by the row sum takes out).  What is left below: a key's absolute error is 2^-25 of values
 // whose largest is 2^(15 - LAG) or more.  bf16 has the exponents of fp32 and needs no shift.
+//
+// What the exponents subtract, m - shift for an offset m (0 for that of a row that has seen nothing), is
+// rounded up, as m is where it is taken from a score (row_max): so an exponent is at most its bound
+// however large the scores are (above 2^23 a rounding is 1 or more, and P would pass 2^16).
 template <bool F16, int LAG>
-__device__ __forceinline__ constexpr float p_shift() {
-  return F16 ? 15.f - LAG : 0.f;
+__device__ __forceinline__ float p_offset(float m) {
+  if (m == -INFINITY) m = 0.f;
+  return F16 ? __fsub_ru(m, 15.f - LAG) : m;
 }
+
+// the running maximum's unit: a raw score's product with scale * log2(e) > 0
+__device__ __forceinline__ float row_max(float top, float scale_log2) { return __fmul_ru(top, scale_log2); }
 
 __device__ __forceinline__ float exp2_mufu(float x) {
   float y;

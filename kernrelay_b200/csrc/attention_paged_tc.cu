@@ -168,22 +168,21 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, fl
         if (!((bits >> e) & 1)) r[c][e] = 0xff800000u;  // -inf
     }
   }
-  constexpr float shift = p_shift<F16, kRescaleLog2>();
   uint32_t pk[32];
   float sum = 0.f;
-  if (has_o) sum = exp_block<F16>(r, scale_log2, (m_run == -INFINITY ? 0.f : m_run) - shift, pk);
+  if (has_o) sum = exp_block<F16>(r, scale_log2, p_offset<F16, kRescaleLog2>(m_run), pk);
   float m4[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) m4[e] = fmaxf(__uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
 #pragma unroll
   for (int e = 4; e < 32; ++e)
     m4[e & 3] = max3(m4[e & 3], __uint_as_float(r[0][e]), __uint_as_float(r[1][e]));
-  const float top = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * scale_log2;
+  const float top = row_max(fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]), scale_log2);
   const bool grow = top - m_run > kRescaleLog2;
   if (!has_o || __any_sync(0xffffffffu, grow)) {
     const float alpha = grow ? exp2_mufu(m_run - top) : 1.f;
     if (grow) m_run = top;
-    sum = exp_block<F16>(r, scale_log2, (m_run == -INFINITY ? 0.f : m_run) - shift, pk);
+    sum = exp_block<F16>(r, scale_log2, p_offset<F16, kRescaleLog2>(m_run), pk);
     l_run *= alpha;
     if (has_o && o_ready()) {
 #pragma unroll 1

@@ -1243,3 +1243,37 @@ def test_step_captured(cuda, krlib, T):
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
         assert torch.equal(k, k1) and torch.equal(v, v1)
         assert not torch.equal(outs[0], outs[1]) and not torch.equal(k, k0)
+
+
+# ---------------------------------------------------------------- very large scores
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("HQ,HKV,D", [(28, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_very_large_scores(cuda, krlib, T, HQ, HKV, D, dtype, sign):
+    """Scores up to 2^27 (in log2 units), where neighbouring fp32 numbers are 8 apart and a maximum's
+    product with the scale is off by as much: one key far above the others is the output, whatever
+    those roundings.  Its probability is rounded once (u), the output once more (u)."""
+    import torch
+    dt, B, n, page, g = _dt(dtype), 40, 700, 16, _gen(T)
+    u = torch.finfo(dt).eps / 2
+    need = -(-n // page)
+    k = torch.empty(1, need, HKV, page, D, dtype=dt, device="cuda").fill_(992 if sign > 0 else 1024)
+    k[0, 30, :, 5] = 1000
+    if sign < 0:
+        k[0, 30, :, 5] = 1000  # the least negative of them
+    v = torch.randn(k.shape, generator=g, device="cuda").to(dt)
+    top = 2.0 ** torch.linspace(18, 27, B * T, device="cuda")
+    scale = D ** -0.5
+    q = (sign * top / (1000 * D * scale * math.log2(math.e)))[:, None, None].expand(B * T, HQ, D).to(dt)
+    assert torch.isfinite(q).all()
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(need, dtype=torch.int32, device="cuda").repeat(B, 1)
+    mask = torch.full((B * T, 2), -1, dtype=torch.int32, device="cuda")
+    out = krlib.attention_paged(q.reshape(B * T, -1), krlib.KVCache(k, v), table, i32([n] * B),
+                                i32([T * i for i in range(B + 1)]), T, scale, mask=mask)
+    torch.cuda.synchronize()
+    ref = v[0, 30, :, 5].double()[None, :, None]
+    got = out.double().view(B * T, HKV, HQ // HKV, D)
+    bad = ~((got - ref).abs() <= (2 * u + u * u + 2.0 ** -20) * ref.abs() + 2.0 ** -25)
+    assert not bad.any(), bad.view(B * T, -1).any(1).nonzero().flatten().tolist()[:9]
